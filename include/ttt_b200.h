@@ -333,6 +333,75 @@ int ttt_mlp_cached_readout(int B, int NH, int NCseg, int CS, int F, int FF,
                            const void* ttt_norm_weight, const void* ttt_norm_bias, int dt_ln,
                            float* out, void* stream);
 
+/* ------------------------------------------------------------------ selective state space scan
+ * A scan of the same kind as the two above for layers whose state decays by an input-dependent
+ * rate: per channel d of D and state n of N,
+ *
+ *   dt = softplus(delta + delta_bias)  (or delta + delta_bias with softplus 0)
+ *   h[t] = exp(dt A) h[t-1] + dt u B[t];  y = <h, C[t]> + Dskip u;  out = y z sigmoid(z)
+ *
+ * u, delta, z, out: [rows, L, D]; B, C: [rows, L, G, N], one row for the D / G channels of a
+ * group; A: [D, N]; Dskip, delta_bias: [D] (or NULL); z may be NULL. u, delta, B, C, z are of
+ * type dt with their last dimension contiguous and the element strides of `strides`:
+ * {u row, u token, delta row, delta token, B row, B token, B group, C row, C token, C group,
+ * z row, z token}. A, Dskip, delta_bias and the states are fp32, out and the gradients of the
+ * activations contiguous. N <= 128.
+ *
+ * Packed sequences: rows = 1 and seq[t] (ttt_sequence_index) names the sequence of token t, or
+ * -1: such tokens give zeros. init / fin: [rows or sequences, D, N] initial state (NULL: zero)
+ * and final state (NULL: not wanted; sequences without a token are left as they were).
+ * saved: ttt_selective_scan_saved_bytes() bytes that the backward reads, or NULL. */
+size_t ttt_selective_scan_fwd_scratch_bytes(int rows, int L, int D, int G, int N);
+size_t ttt_selective_scan_saved_bytes(int rows, int L, int D, int N);
+int ttt_selective_scan_fwd(int rows, int L, int D, int G, int N, const void* u, const void* delta, const void* B,
+                           const void* C, const void* z, int dt, const long long* strides, const float* A,
+                           const float* Dskip, const float* delta_bias, int softplus, const int* seq,
+                           const float* init, float* fin, void* out, float* saved, void* scratch,
+                           size_t scratch_bytes, void* stream);
+/* dout [rows, L, D] contiguous; dfin the gradient of the final state or NULL. du, ddelta, dz
+ * [rows, L, D] and dB, dC [rows, L, G, N] in type dt (dz NULL without z); dinit or NULL (left
+ * as it was for sequences without a token); dparams fp32 [D * (N + 2)]: dA [D, N], the
+ * gradient of Dskip [D], of delta_bias [D]. Sums are taken in one order: results repeat. */
+size_t ttt_selective_scan_bwd_scratch_bytes(int rows, int L, int D, int G, int N);
+int ttt_selective_scan_bwd(int rows, int L, int D, int G, int N, const void* u, const void* delta, const void* B,
+                           const void* C, const void* z, int dt, const long long* strides, const float* A,
+                           const float* Dskip, const float* delta_bias, int softplus, const int* seq,
+                           const float* init, const float* saved, const void* dout, const float* dfin, void* du,
+                           void* ddelta, void* dB, void* dC, void* dz, float* dinit, float* dparams, void* scratch,
+                           size_t scratch_bytes, void* stream);
+/* One token for every row: u, delta, z, out [rows, D], B, C [rows, G, N]; state fp32
+ * [slots, D, N], updated in place (row i uses slot i, or index[i]). A row whose index is
+ * negative is skipped: its output is zero. One whose index is past the last slot or repeats an
+ * earlier row's is not stepped either: its output is NaN. strides: {u row, delta row, B row,
+ * B group, C row, C group, z row, state slot}. */
+int ttt_selective_scan_step(int rows, int D, int G, int N, int slots, const void* u, const void* delta, const void* B,
+                            const void* C, const void* z, int dt, const long long* strides, const float* A,
+                            const float* Dskip, const float* delta_bias, int softplus, const int* index, float* state,
+                            void* out, void* stream);
+
+/* ------------------------------------------------------------------ short causal convolution
+ * p[t] = bias + sum_k w[k] x[t - K + 1 + k] per channel, y = p (act 0) or p sigmoid(p) (act 1),
+ * K = 2 .. 4. x: [rows, L, D] of type dt, element strides {row, token}; w fp32 [D, K]; b fp32 [D]
+ * or NULL; y contiguous. init / fin: the K - 1 rows before a sequence's first token (NULL:
+ * zero) and its last K - 1 rows, [rows or sequences, K - 1, D] in type dt, oldest first.
+ * Packed sequences as for the scan. */
+int ttt_causal_conv_fwd(int rows, int L, int D, int K, const void* x, int dt, const long long* strides, const float* w,
+                        const float* b, int act, const int* seq, const void* init, void* fin, void* y, void* stream);
+/* dparams fp32 [D * (K + 1)]: dw [D, K], then the bias's gradient [D]. */
+size_t ttt_causal_conv_bwd_scratch_bytes(int rows, int L, int D, int K, int dt);
+int ttt_causal_conv_bwd(int rows, int L, int D, int K, const void* x, int dt, const long long* strides, const float* w,
+                        const float* b, int act, const int* seq, const void* init, const void* dy, const void* dfin,
+                        void* dx, void* dinit, float* dparams, void* scratch, size_t scratch_bytes, void* stream);
+/* One token for every row: x, y [rows, D]; state [slots, K - 1, D] of type dt, shifted in place;
+ * index as for ttt_selective_scan_step. strides: {x row, state slot}. */
+int ttt_causal_conv_step(int rows, int D, int K, int slots, const void* x, int dt, const long long* strides,
+                         const float* w, const float* b, int act, const int* index, void* state, void* y, void* stream);
+
+/* seq[t] for t < T: the sequence s with cu_seqlens[s] <= t < cu_seqlens[s + 1], or -1. cu_seqlens:
+ * S + 1 ascending offsets on the device (other values give a wrong seq, never an access out of
+ * bounds). */
+int ttt_sequence_index(int T, int S, const int* cu_seqlens, int* seq, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

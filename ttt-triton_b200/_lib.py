@@ -71,6 +71,17 @@ _SIGNATURES = {
     "ttt_prologue_bwd": ([_I] * 5 + [_P, _I, _L] + [_P] * 4 + [ctypes.c_float] + [_P] * 10, _I),
     "ttt_post_norm_fwd": ([_I] * 4 + [_P, _I, _P, _P, ctypes.c_float, _P, _P], _I),
     "ttt_post_norm_bwd": ([_I] * 4 + [_P, _I, _P, _P, ctypes.c_float] + [_P] * 7, _I),
+    "ttt_selective_scan_fwd_scratch_bytes": ([_I] * 5, _Z),
+    "ttt_selective_scan_saved_bytes": ([_I] * 4, _Z),
+    "ttt_selective_scan_fwd": ([_I] * 5 + [_P] * 5 + [_I] + [_P] * 4 + [_I] + [_P] * 6 + [_Z, _P], _I),
+    "ttt_selective_scan_bwd_scratch_bytes": ([_I] * 5, _Z),
+    "ttt_selective_scan_bwd": ([_I] * 5 + [_P] * 5 + [_I] + [_P] * 4 + [_I] + [_P] * 13 + [_Z, _P], _I),
+    "ttt_selective_scan_step": ([_I] * 5 + [_P] * 5 + [_I] + [_P] * 4 + [_I] + [_P] * 4, _I),
+    "ttt_causal_conv_fwd": ([_I] * 4 + [_P, _I] + [_P] * 3 + [_I] + [_P] * 5, _I),
+    "ttt_causal_conv_bwd_scratch_bytes": ([_I] * 5, _Z),
+    "ttt_causal_conv_bwd": ([_I] * 4 + [_P, _I] + [_P] * 3 + [_I] + [_P] * 8 + [_Z, _P], _I),
+    "ttt_causal_conv_step": ([_I] * 4 + [_P, _I] + [_P] * 3 + [_I] + [_P] * 4, _I),
+    "ttt_sequence_index": ([_I, _I, _P, _P, _P], _I),
     "ttt_mlp_cached_readout": (
         [_I] * 6 + [_P, _I] + [_P, _L, _L] * 4 + [_P, _P, _I, _P, _P],
         _I,

@@ -1,0 +1,290 @@
+"""Functional host side of the selective scan and its causal convolution: shape checks,
+allocation, C-ABI launches, as ``_core`` has them for the TTT scans.
+
+Activations may be strided views (a slice of a wider projection) as long as their last
+dimension is contiguous; others are copied. Nothing here synchronises the device.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from _core import _on_tensor_device
+from _lib import check, dtype_code, lib, ptr, require_cuda, stream_of
+
+MAX_STATES = 128
+
+
+def _rows(t):
+    """t with a contiguous last dimension."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _strides(*values):
+    return (ctypes.c_longlong * len(values))(*values)
+
+
+def _f32(t):
+    if t is None:
+        return None
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
+
+
+def _same(ref, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.dtype != ref.dtype:
+            raise ValueError(f"{name} must have dtype {ref.dtype}, got {t.dtype}")
+
+
+def _shaped(name, t, shape):
+    if t is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+
+
+@_on_tensor_device
+def sequence_index(cu_seqlens, T):
+    """Each token's sequence, int32 [T], from S + 1 ascending offsets; -1 outside of all."""
+    seq = torch.empty(T, device=cu_seqlens.device, dtype=torch.int32)
+    if T:
+        check(lib.ttt_sequence_index(T, cu_seqlens.numel() - 1, ptr(cu_seqlens), ptr(seq), stream_of(seq)),
+              "ttt_sequence_index")
+    return seq
+
+
+def packed(cu_seqlens, x):
+    """(number of sequences, checked int32 offsets) of a batch of shape x.shape[:2]."""
+    if cu_seqlens is None:
+        return x.shape[0], None
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.is_floating_point():
+        raise ValueError("cu_seqlens must hold the S + 1 >= 2 offsets of S packed sequences")
+    if x.shape[0] != 1:
+        raise ValueError(f"packed sequences lie in one row: expected a batch of 1, got {x.shape[0]}")
+    return cu_seqlens.numel() - 1, cu_seqlens.to(torch.int32).contiguous()
+
+
+# --------------------------------------------------------------------------- selective scan
+def check_scan(u, delta, A, B, C, D, z, delta_bias, init, nseq):
+    require_cuda(*(t for t in (u, delta, A, B, C, D, z, delta_bias, init) if t is not None))
+    dtype_code(u)
+    if u.dim() != 3:
+        raise ValueError(f"u must be [B, L, D], got shape {tuple(u.shape)}")
+    rows, L, W = u.shape
+    if A.dim() != 2 or A.shape[0] != W or A.shape[1] < 1:
+        raise ValueError(f"A must be [{W}, N], got {tuple(A.shape)}")
+    N = A.shape[1]
+    if N > MAX_STATES:
+        raise ValueError(f"{N} states per channel: at most {MAX_STATES} are supported")
+    if W < 1:
+        raise ValueError("the scan needs at least one channel")
+    _shaped("delta", delta, u.shape)
+    _shaped("z", z, u.shape)
+    if B.dim() != 4 or tuple(B.shape[:2]) != (rows, L) or B.shape[3] != N or B.shape[2] < 1 or W % B.shape[2]:
+        raise ValueError(f"B must be [{rows}, {L}, {N}] or [{rows}, {L}, G, {N}] with G dividing {W}, "
+                         f"got {tuple(B.shape)}")
+    _shaped("C", C, B.shape)
+    _shaped("D", D, (W,))
+    _shaped("delta_bias", delta_bias, (W,))
+    _shaped("initial_state", init, (nseq, W, N))
+    _same(u, delta=delta, B=B, C=C, z=z)
+
+
+def _scan_args(u, delta, A, B, C, D, z, delta_bias, softplus):
+    rows, L, W = u.shape
+    st = _strides(u.stride(0), u.stride(1), delta.stride(0), delta.stride(1), B.stride(0), B.stride(1), B.stride(2),
+                  C.stride(0), C.stride(1), C.stride(2), *(z.stride()[:2] if z is not None else (0, 0)))
+    return (rows, L, W, B.shape[2], A.shape[1], ptr(u), ptr(delta), ptr(B), ptr(C), ptr(z), dtype_code(u), st, ptr(A),
+            ptr(D), ptr(delta_bias), int(softplus))
+
+
+@_on_tensor_device
+def selective_scan_forward(u, delta, A, B, C, D, z, delta_bias, softplus, init, seq, nseq, want_final, for_backward):
+    """Returns (out [B, L, D] in u's dtype, final state fp32 or None, saved states or None).
+    u, delta, B, C, z with contiguous last dimensions; A, D, delta_bias, init fp32 contiguous."""
+    rows, L, W = u.shape
+    N = A.shape[1]
+    dev = u.device
+    out = torch.empty(rows, L, W, device=dev, dtype=u.dtype)
+    fin = saved = None
+    if want_final:
+        if seq is None and L:
+            fin = torch.empty(nseq, W, N, device=dev, dtype=torch.float32)
+        else:  # sequences without a token keep their initial state
+            fin = init.clone() if init is not None else torch.zeros(nseq, W, N, device=dev, dtype=torch.float32)
+    if rows * L == 0:
+        return out, fin, torch.empty(0, device=dev) if for_backward else None
+    args = _scan_args(u, delta, A, B, C, D, z, delta_bias, softplus)
+    if for_backward:
+        saved = torch.empty(lib.ttt_selective_scan_saved_bytes(rows, L, W, N) // 4, device=dev, dtype=torch.float32)
+    nbytes = lib.ttt_selective_scan_fwd_scratch_bytes(rows, L, W, args[3], N)
+    scratch = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+    check(lib.ttt_selective_scan_fwd(*args, ptr(seq), ptr(init), ptr(fin), ptr(out), ptr(saved), ptr(scratch), nbytes,
+                                     stream_of(u)), "ttt_selective_scan_fwd")
+    return out, fin, saved
+
+
+@_on_tensor_device
+def selective_scan_backward(u, delta, A, B, C, D, z, delta_bias, softplus, init, seq, saved, dout, dfin, want_dinit):
+    """Returns (du, ddelta, dA, dB, dC, dD, dz or None, ddelta_bias, dinit or None); the
+    gradients of A, D, delta_bias and the state in fp32, the others in u's dtype."""
+    rows, L, W = u.shape
+    G, N = B.shape[2], A.shape[1]
+    dev, dt = u.device, u.dtype
+    du, ddelta = (torch.empty(rows, L, W, device=dev, dtype=dt) for _ in range(2))
+    dz = torch.empty(rows, L, W, device=dev, dtype=dt) if z is not None else None
+    dB, dC = (torch.empty(rows, L, G, N, device=dev, dtype=dt) for _ in range(2))
+    dinit = None
+    if want_dinit:
+        dinit = dfin.clone() if dfin is not None else torch.zeros(init.shape, device=dev, dtype=torch.float32)
+    if rows * L == 0:
+        zeros = torch.zeros(W * (N + 2), device=dev, dtype=torch.float32)
+        return du, ddelta, zeros[:W * N].view(W, N), dB, dC, zeros[-2 * W:-W], dz, zeros[-W:], dinit
+    dparams = torch.empty(W * (N + 2), device=dev, dtype=torch.float32)
+    nbytes = lib.ttt_selective_scan_bwd_scratch_bytes(rows, L, W, G, N)
+    scratch = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    check(lib.ttt_selective_scan_bwd(*_scan_args(u, delta, A, B, C, D, z, delta_bias, softplus), ptr(seq), ptr(init),
+                                     ptr(saved), ptr(dout), ptr(dfin), ptr(du), ptr(ddelta), ptr(dB), ptr(dC), ptr(dz),
+                                     ptr(dinit), ptr(dparams), ptr(scratch), nbytes, stream_of(u)),
+          "ttt_selective_scan_bwd")
+    return du, ddelta, dparams[:W * N].view(W, N), dB, dC, dparams[W * N:W * (N + 1)], dz, dparams[W * (N + 1):], dinit
+
+
+def _check_step(state, index, rows, inputs, shape):
+    """The carried state and the slots of a single-token call."""
+    if state.dim() != 3 or tuple(state.shape[1:]) != shape:
+        raise ValueError(f"the state must be [slots, {shape[0]}, {shape[1]}], got {tuple(state.shape)}")
+    if state.stride(2) != 1 or state.stride(1) != shape[1]:
+        raise ValueError("the state is updated in place: each slot must be contiguous")
+    if state.shape[0] > 1 and state.stride(0) < shape[0] * shape[1]:
+        raise ValueError("the state's slots must not overlap")
+    if index is None:
+        if state.shape[0] != rows:
+            raise ValueError(f"{rows} rows need a state of {rows} slots or state_indices, got {state.shape[0]} slots")
+    elif index.dim() != 1 or index.numel() != rows or index.dtype != torch.int32 or not index.is_contiguous():
+        raise ValueError(f"state_indices must be contiguous int32 [{rows}]")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in inputs if t is not None):
+        raise RuntimeError("the single-token step has no gradient: call it under torch.no_grad()")
+
+
+@_on_tensor_device
+def selective_scan_step(state, u, delta, A, B, C, D, z, delta_bias, softplus, index):
+    """One token per row: out [B, D]; state [slots, D, N] fp32 updated in place."""
+    inputs = (state, u, delta, A, B, C, D, z, delta_bias)
+    require_cuda(*(t for t in (*inputs, index) if t is not None))
+    if u.dim() != 2:
+        raise ValueError(f"u must be [B, D], got shape {tuple(u.shape)}")
+    rows, W = u.shape
+    if A.dim() != 2 or A.shape[0] != W or not 1 <= A.shape[1] <= MAX_STATES:
+        raise ValueError(f"A must be [{W}, N] with N from 1 to {MAX_STATES}, got {tuple(A.shape)}")
+    N = A.shape[1]
+    _shaped("delta", delta, u.shape)
+    _shaped("z", z, u.shape)
+    if B.dim() != 3 or B.shape[0] != rows or B.shape[2] != N or B.shape[1] < 1 or W % B.shape[1]:
+        raise ValueError(f"B must be [{rows}, {N}] or [{rows}, G, {N}] with G dividing {W}, got {tuple(B.shape)}")
+    _shaped("C", C, B.shape)
+    _shaped("D", D, (W,))
+    _shaped("delta_bias", delta_bias, (W,))
+    _same(u, delta=delta, B=B, C=C, z=z)
+    if state.dtype != torch.float32:
+        raise ValueError(f"the state must be float32, got {state.dtype}")
+    _check_step(state, index, rows, inputs, (W, N))
+    out = torch.empty(rows, W, device=u.device, dtype=u.dtype)
+    if rows == 0:
+        return out
+    u, delta, B, C = _rows(u), _rows(delta), _rows(B), _rows(C)
+    z = _rows(z) if z is not None else None
+    A, D, delta_bias = _f32(A), _f32(D), _f32(delta_bias)
+    st = _strides(u.stride(0), delta.stride(0), B.stride(0), B.stride(1), C.stride(0), C.stride(1),
+                  z.stride(0) if z is not None else 0, state.stride(0))
+    check(lib.ttt_selective_scan_step(rows, W, B.shape[1], N, state.shape[0], ptr(u), ptr(delta), ptr(B), ptr(C), ptr(z),
+                                      dtype_code(u), st, ptr(A), ptr(D), ptr(delta_bias), int(softplus), ptr(index),
+                                      ptr(state), ptr(out), stream_of(u)), "ttt_selective_scan_step")
+    return out
+
+
+# --------------------------------------------------------------------------- causal convolution
+def _act_code(activation):
+    if activation not in (None, "silu"):
+        raise ValueError(f"activation must be None or 'silu', got {activation!r}")
+    return int(activation == "silu")
+
+
+def _check_taps(weight, bias, W):
+    if weight.dim() != 2 or weight.shape[0] != W or not 2 <= weight.shape[1] <= 4:
+        raise ValueError(f"weight must be [{W}, K] with 2 to 4 taps, got {tuple(weight.shape)}")
+    _shaped("bias", bias, (W,))
+    return weight.shape[1]
+
+
+def check_conv(x, weight, bias, init, nseq):
+    require_cuda(*(t for t in (x, weight, bias, init) if t is not None))
+    dtype_code(x)
+    if x.dim() != 3 or x.shape[2] < 1:
+        raise ValueError(f"x must be [B, L, D], got shape {tuple(x.shape)}")
+    W = x.shape[2]
+    K = _check_taps(weight, bias, W)
+    _shaped("initial_state", init, (nseq, K - 1, W))
+    _same(x, initial_state=init)
+    return K
+
+
+@_on_tensor_device
+def causal_conv_forward(x, w, b, act, init, seq, nseq, want_final):
+    """Returns (y [B, L, D], final state [sequences, K - 1, D] or None), both in x's dtype."""
+    rows, L, W = x.shape
+    K = w.shape[1]
+    y = torch.empty(rows, L, W, device=x.device, dtype=x.dtype)
+    fin = None
+    if want_final:
+        if seq is None and L:
+            fin = torch.empty(nseq, K - 1, W, device=x.device, dtype=x.dtype)
+        else:
+            fin = init.clone() if init is not None else torch.zeros(nseq, K - 1, W, device=x.device, dtype=x.dtype)
+    if rows * L == 0:
+        return y, fin
+    check(lib.ttt_causal_conv_fwd(rows, L, W, K, ptr(x), dtype_code(x), _strides(x.stride(0), x.stride(1)), ptr(w),
+                                  ptr(b), act, ptr(seq), ptr(init), ptr(fin), ptr(y), stream_of(x)),
+          "ttt_causal_conv_fwd")
+    return y, fin
+
+
+@_on_tensor_device
+def causal_conv_backward(x, w, b, act, init, seq, dy, dfin, want_dinit):
+    """Returns (dx, dw fp32, db fp32, dinit or None)."""
+    rows, L, W = x.shape
+    K = w.shape[1]
+    dx = torch.empty(rows, L, W, device=x.device, dtype=x.dtype)
+    dinit = None
+    if want_dinit:
+        dinit = dfin.clone() if dfin is not None else torch.zeros(init.shape, device=x.device, dtype=x.dtype)
+    if rows * L == 0:
+        return dx, torch.zeros_like(w), torch.zeros(W, device=x.device, dtype=torch.float32), dinit
+    dparams = torch.empty(W * (K + 1), device=x.device, dtype=torch.float32)
+    nbytes = lib.ttt_causal_conv_bwd_scratch_bytes(rows, L, W, K, dtype_code(x))
+    scratch = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+    check(lib.ttt_causal_conv_bwd(rows, L, W, K, ptr(x), dtype_code(x), _strides(x.stride(0), x.stride(1)), ptr(w),
+                                  ptr(b), act, ptr(seq), ptr(init), ptr(dy), ptr(dfin), ptr(dx), ptr(dinit),
+                                  ptr(dparams), ptr(scratch), nbytes, stream_of(x)), "ttt_causal_conv_bwd")
+    return dx, dparams[:W * K].view(W, K), dparams[W * K:], dinit
+
+
+@_on_tensor_device
+def causal_conv_step(x, state, weight, bias, activation, index):
+    """One token per row: y [B, D]; state [slots, K - 1, D] shifted in place."""
+    require_cuda(*(t for t in (x, state, weight, bias, index) if t is not None))
+    act = _act_code(activation)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"x must be [B, D], got shape {tuple(x.shape)}")
+    rows, W = x.shape
+    K = _check_taps(weight, bias, W)
+    _same(x, conv_state=state)
+    _check_step(state, index, rows, (x, state, weight, bias), (K - 1, W))
+    y = torch.empty(rows, W, device=x.device, dtype=x.dtype)
+    if rows == 0:
+        return y
+    x, w, b = _rows(x), _f32(weight), _f32(bias)
+    check(lib.ttt_causal_conv_step(rows, W, K, state.shape[0], ptr(x), dtype_code(x),
+                                   _strides(x.stride(0), state.stride(0)), ptr(w), ptr(b), act, ptr(index), ptr(state),
+                                   ptr(y), stream_of(x)), "ttt_causal_conv_step")
+    return y

@@ -1,0 +1,468 @@
+// Selective state space scan, forward: prompts, packed prompts and the training forward, and
+// the single-token step. The recurrence is in selective_scan.cuh.
+//
+// A channel's N states are split over LN threads, NPT in each, and stay in registers while the
+// CTA walks the time axis tile by tile: a tile's step sizes and inputs are worked out once per
+// (token, channel) into shared memory, then every thread runs its states through the tile's
+// tokens, then the threads add the partial outputs of their channel, apply the skip and the
+// gate and write. One exponential per (token, channel, state) is what bounds it.
+//
+// With few channels in all, the time axis is split into pieces: a first pass finds each
+// piece's end state from zero and the sum of its step sizes (its whole decay is
+// exp(A * sum)), a second runs over the pieces, and the main pass starts each piece from
+// the state that enters it.
+#include "selective_scan.cuh"
+
+namespace ttt {
+namespace scan {
+
+template <int LN, int NPT>
+struct Fwd {
+  static constexpr int THREADS = 128;
+  static constexpr int DT = THREADS / LN;            // channels of a CTA
+  static constexpr int NP = LN * NPT;                // states, padded
+  static constexpr int TT = LN >= 4 ? 32 : 8 * LN;   // tokens of a tile
+  static constexpr int PAIRS = TT * DT / THREADS;    // (token, channel) pairs of a thread
+  struct Smem {
+    float B[TT * NP], C[TT * NP];
+    float2 d[TT * DT];      // step size, step size * input
+    float y[TT * THREADS];  // partial outputs
+    SeqMask m;
+  };
+};
+
+template <typename T, int LN, int NPT>
+__global__ void __launch_bounds__(128) scan_fwd_kernel(const __grid_constant__ Params p) {
+  using F = Fwd<LN, NPT>;
+  extern __shared__ __align__(16) unsigned char raw_smem[];
+  auto& s = *reinterpret_cast<typename F::Smem*>(raw_smem);
+  const Where w = where<F::DT>(p);
+  const int tid = threadIdx.x, nl = tid % LN, cl = tid / LN;
+  const int n0 = nl * NPT;
+  const int d = w.g * p.Dg + w.d0 + cl;              // this thread's channel in the recurrence
+  const bool on = w.d0 + cl < p.Dg;
+  const int pc = tid % F::DT, pd = w.g * p.Dg + w.d0 + pc;  // and in the element-wise passes
+  const bool pon = w.d0 + pc < p.Dg;
+  const int tbeg = w.piece * p.chunk, tend = min(p.L, tbeg + p.chunk);
+
+  float A2[NPT], h[NPT];
+  load_states<NPT>(p.A, d, n0, p.N, on, A2);
+#pragma unroll
+  for (int i = 0; i < NPT; ++i) A2[i] *= kLog2e;
+  if (p.nchunks > 1)
+    load_states<NPT>(p.cstate + ((long long)w.row * p.nchunks + w.piece) * p.D * p.N, d, n0, p.N, on, h);
+  else if (p.init && !p.seq)
+    load_states<NPT>(p.init + (long long)w.row * p.D * p.N, d, n0, p.N, on, h);
+  else
+    load_states<NPT>(p.A, d, n0, p.N, false, h);
+  const float skip = pon && p.Dskip ? p.Dskip[pd] : 0.f, bias = pon && p.bias ? p.bias[pd] : 0.f;
+  const T* u = static_cast<const T*>(p.u) + w.row * p.u_b + pd;
+  const T* delta = static_cast<const T*>(p.delta) + w.row * p.delta_b + pd;
+  const T* z = p.z ? static_cast<const T*>(p.z) + w.row * p.z_b + pd : nullptr;
+  const T* B = static_cast<const T*>(p.B) + w.row * p.B_b + w.g * p.B_g;
+  const T* C = static_cast<const T*>(p.C) + w.row * p.C_b + w.g * p.C_g;
+  T* out = static_cast<T*>(p.out) + (long long)w.row * p.L * p.D + pd;
+  const int every = 64 / NPT;
+
+  for (int t0 = tbeg; t0 < tend; t0 += F::TT) {
+    float uu[F::PAIRS], zz[F::PAIRS];
+    if (p.seq) stage_masks<F::TT>(&s.m, p.seq, t0, tend, p.L);
+#pragma unroll
+    for (int k = 0; k < F::PAIRS; ++k) {
+      const int t = tid / F::DT + k * LN, tok = t0 + t;
+      float dt = 0.f;
+      uu[k] = zz[k] = 0.f;
+      if (pon && tok < tend && !(p.seq && p.seq[tok] < 0)) {
+        uu[k] = to_f(u[tok * p.u_l]);
+        dt = step_size(p, to_f(delta[tok * p.delta_l]) + bias);
+        if (z) zz[k] = to_f(z[tok * p.z_l]);
+      }
+      s.d[t * F::DT + pc] = make_float2(dt, dt * uu[k]);
+    }
+    stage_rows<T, F::NP, F::TT, F::THREADS>(s.B, B, p.B_l, t0, tend, p.N, p.seq);
+    stage_rows<T, F::NP, F::TT, F::THREADS>(s.C, C, p.C_l, t0, tend, p.N, p.seq);
+    __syncthreads();
+
+    for (int t = 0; t < F::TT; ++t) {
+      if (t0 + t >= tend) break;
+      if (p.hsave && (t0 + t) % every == 0)
+        store_states<NPT>(p.hsave + ((long long)w.row * p.nsave + (t0 + t) / every) * p.D * p.N, d, n0, p.N, on, h);
+      if (p.seq && (s.m.start >> t & 1)) {
+        const int q = p.seq[t0 + t];
+        load_states<NPT>(p.init + (long long)q * p.D * p.N, d, n0, p.N, on && q >= 0 && p.init, h);
+      }
+      const float2 dd = s.d[t * F::DT + cl];
+      float y = 0.f;
+#pragma unroll
+      for (int i = 0; i < NPT; ++i) {
+        h[i] = fmaf(ex2(dd.x * A2[i]), h[i], dd.y * s.B[t * F::NP + n0 + i]);
+        y = fmaf(h[i], s.C[t * F::NP + n0 + i], y);
+      }
+      s.y[t * F::THREADS + tid] = y;
+      if (p.seq && p.fin && (s.m.end >> t & 1)) {
+        const int q = p.seq[t0 + t];
+        store_states<NPT>(p.fin + (long long)q * p.D * p.N, d, n0, p.N, on && q >= 0, h);
+      }
+    }
+    __syncthreads();
+
+#pragma unroll
+    for (int k = 0; k < F::PAIRS; ++k) {
+      const int t = tid / F::DT + k * LN, tok = t0 + t;
+      if (pon && tok < tend) {
+        float y = 0.f;
+#pragma unroll
+        for (int j = 0; j < LN; ++j) y += s.y[t * F::THREADS + pc * LN + j];
+        y = fmaf(skip, uu[k], y);
+        if (z) y *= zz[k] * sigmoid(zz[k]);
+        if (p.seq && !(s.m.in >> t & 1)) y = 0.f;  // a token of no sequence
+        out[(long long)tok * p.D] = from_f<T>(y);
+      }
+    }
+    if (p.seq) __syncthreads();  // the masks are written again
+  }
+  if (!p.seq && p.fin && tend == p.L)
+    store_states<NPT>(p.fin + (long long)w.row * p.D * p.N, d, n0, p.N, on, h);
+}
+
+// A piece's end state from zero (REV: the carry that leaves its first token from zero at its
+// last), and the sum of its step sizes.
+template <typename T, int LN, int NPT, bool REV>
+__global__ void __launch_bounds__(128) scan_chunk_kernel(const __grid_constant__ Params p) {
+  using F = Fwd<LN, NPT>;
+  extern __shared__ __align__(16) unsigned char raw_smem[];
+  auto& s = *reinterpret_cast<typename F::Smem*>(raw_smem);
+  const Where w = where<F::DT>(p);
+  const int tid = threadIdx.x, nl = tid % LN, cl = tid / LN;
+  const int n0 = nl * NPT;
+  const int d = w.g * p.Dg + w.d0 + cl;
+  const bool on = w.d0 + cl < p.Dg;
+  const int pc = tid % F::DT, pd = w.g * p.Dg + w.d0 + pc;
+  const bool pon = w.d0 + pc < p.Dg;
+  const int tbeg = w.piece * p.chunk, tend = min(p.L, tbeg + p.chunk);
+
+  float A2[NPT], h[NPT], sum = 0.f;
+  load_states<NPT>(p.A, d, n0, p.N, on, A2);
+#pragma unroll
+  for (int i = 0; i < NPT; ++i) A2[i] *= kLog2e, h[i] = 0.f;
+  const float bias = pon && p.bias ? p.bias[pd] : 0.f;
+  const T* delta = static_cast<const T*>(p.delta) + w.row * p.delta_b + pd;
+  // what drives the recurrence: u and B, or dout (gated) and C
+  const T* v = REV ? static_cast<const T*>(p.dout) + (long long)w.row * p.L * p.D + pd
+                   : static_cast<const T*>(p.u) + w.row * p.u_b + pd;
+  const long long v_l = REV ? p.D : p.u_l;
+  const T* z = REV && p.z ? static_cast<const T*>(p.z) + w.row * p.z_b + pd : nullptr;
+  const T* R = REV ? static_cast<const T*>(p.C) + w.row * p.C_b + w.g * p.C_g
+                   : static_cast<const T*>(p.B) + w.row * p.B_b + w.g * p.B_g;
+  const long long r_l = REV ? p.C_l : p.B_l;
+  const float* edge = REV ? p.dfin : p.init;
+
+  const int ntiles = (tend - tbeg + F::TT - 1) / F::TT;
+  for (int k0 = 0; k0 < ntiles; ++k0) {
+    const int t0 = tbeg + (REV ? ntiles - 1 - k0 : k0) * F::TT;
+    if (p.seq) stage_masks<F::TT>(&s.m, p.seq, t0, tend, p.L);
+#pragma unroll
+    for (int k = 0; k < F::PAIRS; ++k) {
+      const int t = tid / F::DT + k * LN, tok = t0 + t;
+      float dt = 0.f, x = 0.f;
+      if (pon && tok < tend && !(p.seq && p.seq[tok] < 0)) {
+        dt = step_size(p, to_f(delta[tok * p.delta_l]) + bias);
+        x = to_f(v[tok * v_l]);
+        if (REV && z) {
+          const float zz = to_f(z[tok * p.z_l]);
+          x *= zz * sigmoid(zz);
+        }
+        if (!REV) x *= dt;
+      }
+      s.d[t * F::DT + pc] = make_float2(dt, x);
+    }
+    stage_rows<T, F::NP, F::TT, F::THREADS>(s.B, R, r_l, t0, tend, p.N, p.seq);
+    __syncthreads();
+    for (int k = 0; k < F::TT; ++k) {
+      const int t = REV ? F::TT - 1 - k : k;
+      if (t0 + t >= tend) continue;
+      if (p.seq && ((REV ? s.m.end : s.m.start) >> t & 1)) {
+        const int q = p.seq[t0 + t];
+        load_states<NPT>(edge + (long long)q * p.D * p.N, d, n0, p.N, on && q >= 0 && edge, h);
+      }
+      const float2 dd = s.d[t * F::DT + cl];
+      sum += dd.x;
+#pragma unroll
+      for (int i = 0; i < NPT; ++i) {
+        const float a = ex2(dd.x * A2[i]), x = dd.y * s.B[t * F::NP + n0 + i];
+        h[i] = REV ? a * (h[i] + x) : fmaf(a, h[i], x);
+      }
+    }
+    __syncthreads();
+  }
+  const long long at = (long long)w.row * p.nchunks + w.piece;
+  store_states<NPT>(p.cstate + at * p.D * p.N, d, n0, p.N, on, h);
+  if (on && nl == 0) p.csum[at * p.D + d] = sum;
+}
+
+// Turns the pieces' end states into the states that enter them, in place. One thread per
+// (row, channel, state).
+template <bool REV>
+__global__ void __launch_bounds__(256) scan_carry_kernel(const __grid_constant__ Params p) {
+  const long long DN = (long long)p.D * p.N, i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= DN * p.rows) return;
+  const int row = i / DN;
+  const long long e = i - row * DN;
+  const int d = e / p.N;
+  const float A2 = p.A[e] * kLog2e;
+  const float* edge = REV ? p.dfin : p.init;
+  float h = edge && !p.seq ? edge[row * DN + e] : 0.f;
+  for (int k = 0; k < p.nchunks; ++k) {
+    const int c = REV ? p.nchunks - 1 - k : k;
+    const long long at = (long long)row * p.nchunks + c;
+    bool cut = false;
+    if (p.seq) {  // a sequence that starts (ends) in the piece cuts what follows off from what came before
+      const int t0 = c * p.chunk, t1 = min(p.L, t0 + p.chunk);
+      cut = REV ? t1 >= p.L || p.seq[t1] != p.seq[t0] : t0 == 0 || p.seq[t0 - 1] != p.seq[t1 - 1];
+    }
+    float* q = p.cstate + at * DN + e;
+    const float own = *q;
+    *q = h;
+    h = cut ? own : fmaf(ex2(A2 * p.csum[at * p.D + d]), h, own);
+  }
+}
+
+// ------------------------------------------------------------------------------ single token
+struct StepParams {
+  int rows, D, G, N, Dg, slots;
+  const void *u, *delta, *B, *C, *z;
+  long long u_b, delta_b, B_b, B_g, C_b, C_g, z_b, state_b;
+  const float *A, *Dskip, *bias;
+  int softplus;
+  const int* index;  // each row's slot of the state, or NULL: row i has slot i
+  float* state;      // [slots, D, N]
+  void* out;         // [rows, D]
+};
+
+template <typename T, int LN, int NPT>
+__global__ void __launch_bounds__(128) scan_step_kernel(const __grid_constant__ StepParams p) {
+  constexpr int DT = 128 / LN;
+  const int tid = threadIdx.x, nl = tid % LN, n0 = nl * NPT;
+  const int tiles = (p.D + DT - 1) / DT;
+  const int row = blockIdx.x / tiles, d = (blockIdx.x - row * tiles) * DT + tid / LN;
+  const bool on = d < p.D;
+  const int ok = slot_state(p.index, row, p.slots);
+  if (ok <= 0) {
+    if (on && nl == 0)
+      static_cast<T*>(p.out)[(long long)row * p.D + d] = from_f<T>(ok < 0 ? __int_as_float(0x7fffffff) : 0.f);
+    return;
+  }
+  float y = 0.f, u = 0.f, z = 0.f;
+  if (on) {
+    float* state = p.state + (long long)(p.index ? p.index[row] : row) * p.state_b;
+    const int g = d / p.Dg;
+    u = to_f(static_cast<const T*>(p.u)[row * p.u_b + d]);
+    if (p.z) z = to_f(static_cast<const T*>(p.z)[row * p.z_b + d]);
+    const float dt = p.softplus
+                         ? softplus(to_f(static_cast<const T*>(p.delta)[row * p.delta_b + d]) + (p.bias ? p.bias[d] : 0.f))
+                         : to_f(static_cast<const T*>(p.delta)[row * p.delta_b + d]) + (p.bias ? p.bias[d] : 0.f);
+    const T* B = static_cast<const T*>(p.B) + row * p.B_b + g * p.B_g;
+    const T* C = static_cast<const T*>(p.C) + row * p.C_b + g * p.C_g;
+#pragma unroll
+    for (int i = 0; i < NPT; ++i) {
+      const int n = n0 + i;
+      if (n < p.N) {
+        const long long e = (long long)d * p.N + n;
+        const float h = fmaf(ex2(dt * (p.A[e] * kLog2e)), state[e], dt * u * to_f(B[n]));
+        state[e] = h;
+        y = fmaf(h, to_f(C[n]), y);
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < LN; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+  if (on && nl == 0) {
+    if (p.Dskip) y = fmaf(p.Dskip[d], u, y);
+    if (p.z) y *= z * sigmoid(z);
+    static_cast<T*>(p.out)[(long long)row * p.D + d] = from_f<T>(y);
+  }
+}
+
+// Sequence of each token from the sequences' ends: the last s with cu[s] <= t, if t < cu[s + 1].
+__global__ void __launch_bounds__(256) sequence_index_kernel(int T, int S, const int* cu, int* seq) {
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= T) return;
+  int lo = 0, hi = S;  // cu[lo] <= t < cu[hi], were cu[0] <= t < cu[S]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  seq[t] = cu[lo] <= t && t < cu[lo + 1] ? lo : -1;
+}
+
+// ------------------------------------------------------------------------------ host
+template <typename T>
+static int launch_fwd(Params p, cudaStream_t st, const char* who) {
+  return dispatch(p.N, [&](auto ln, auto npt) {
+    using F = Fwd<decltype(ln)::value, decltype(npt)::value>;
+    auto kernel = scan_fwd_kernel<T, decltype(ln)::value, decltype(npt)::value>;
+    Params q = p;
+    q.tiles = (p.Dg + F::DT - 1) / F::DT;
+    const int rc = prepare_smem(kernel, sizeof(typename F::Smem), who);
+    if (rc) return rc;
+    const long long grid = (long long)q.tiles * q.G * q.nchunks * q.rows;
+    TTT_REQUIRE(grid < (1LL << 31), TTT_ERR_SHAPE, "%s: %lld blocks are too many", who, grid);
+    kernel<<<(unsigned)grid, F::THREADS, sizeof(typename F::Smem), st>>>(q);
+    return check_launch(who);
+  });
+}
+
+template <typename T, bool REV>
+static int launch_chunks(Params p, cudaStream_t st, const char* who) {
+  return dispatch(p.N, [&](auto ln, auto npt) {
+    using F = Fwd<decltype(ln)::value, decltype(npt)::value>;
+    auto kernel = scan_chunk_kernel<T, decltype(ln)::value, decltype(npt)::value, REV>;
+    Params q = p;
+    q.tiles = (p.Dg + F::DT - 1) / F::DT;
+    int rc = prepare_smem(kernel, sizeof(typename F::Smem), who);
+    if (rc) return rc;
+    const long long grid = (long long)q.tiles * q.G * q.nchunks * q.rows;
+    TTT_REQUIRE(grid < (1LL << 31), TTT_ERR_SHAPE, "%s: %lld blocks are too many", who, grid);
+    kernel<<<(unsigned)grid, F::THREADS, sizeof(typename F::Smem), st>>>(q);
+    if ((rc = check_launch(who))) return rc;
+    scan_carry_kernel<REV><<<(unsigned)(((long long)p.rows * p.D * p.N + 255) / 256), 256, 0, st>>>(q);
+    return check_launch(who);
+  });
+}
+
+int chunk_states(const Params& p, int dt, bool rev, cudaStream_t st, const char* who) {
+  if (rev)
+    return dt == DT_BF16  ? launch_chunks<__nv_bfloat16, true>(p, st, who)
+           : dt == DT_F16 ? launch_chunks<__half, true>(p, st, who)
+                          : launch_chunks<float, true>(p, st, who);
+  return dt == DT_BF16  ? launch_chunks<__nv_bfloat16, false>(p, st, who)
+         : dt == DT_F16 ? launch_chunks<__half, false>(p, st, who)
+                        : launch_chunks<float, false>(p, st, who);
+}
+
+// Pieces of the time axis: as many as bring the device about two full waves of warps, no
+// piece under 64 tokens.
+int pieces(int rows, int L, int D, int N) {
+  const Shape s = shape_of(N);
+  const long long warps = ((long long)rows * D * s.LN + 31) / 32, want = (long long)sm_count() * 32;
+  if (warps >= want / 2 || L < 256) return 1;
+  long long n = (want + warps - 1) / warps;
+  if (n > L / 64) n = L / 64;
+  return n < 1 ? 1 : (int)n;
+}
+// Tokens of a piece: a multiple of 64, so that tiles and saved states of every shape start on it.
+int piece_tokens(int L, int n) { return ((L + n - 1) / n + 63) / 64 * 64; }
+
+int check_sizes(const char* who, int rows, int L, int D, int G, int N, int dt) {
+  TTT_REQUIRE(rows >= 1 && L >= 1 && D >= 1 && G >= 1 && N >= 1, TTT_ERR_SHAPE,
+              "%s: sizes must be positive, got rows=%d L=%d D=%d G=%d N=%d", who, rows, L, D, G, N);
+  TTT_REQUIRE(D % G == 0, TTT_ERR_SHAPE, "%s: %d channels do not divide into %d groups", who, D, G);
+  TTT_REQUIRE(N <= kMaxStates, TTT_ERR_SHAPE, "%s: %d states per channel, at most %d", who, N, kMaxStates);
+  TTT_REQUIRE((long long)rows * L < (1LL << 31) - 4096, TTT_ERR_SHAPE, "%s: %lld tokens are too many", who,
+              (long long)rows * L);
+  TTT_REQUIRE((long long)rows * D * N < (1LL << 38), TTT_ERR_SHAPE, "%s: too many states", who);
+  TTT_REQUIRE(valid_dtype(dt), TTT_ERR_DTYPE, "%s: bad dtype code %d", who, dt);
+  return TTT_OK;
+}
+
+// Splits the time axis and lays the scratch out; `extra` bytes of the caller come first.
+int plan(Params& p, void* scratch, size_t scratch_bytes, size_t extra, const char* who) {
+  const int n = pieces(p.rows, p.L, p.D, p.N);
+  p.chunk = n > 1 ? piece_tokens(p.L, n) : p.L;
+  p.nchunks = (p.L + p.chunk - 1) / p.chunk;
+  const size_t states = (size_t)p.rows * p.nchunks * p.D;
+  const size_t need = extra + (p.nchunks > 1 ? states * (p.N + 1) * sizeof(float) : 0);
+  TTT_REQUIRE(!need || (scratch && scratch_bytes >= need), TTT_ERR_SCRATCH, "%s: scratch of %zu bytes needed, got %zu",
+              who, need, scratch ? scratch_bytes : (size_t)0);
+  if (p.nchunks > 1) {
+    p.cstate = reinterpret_cast<float*>(static_cast<char*>(scratch) + extra);
+    p.csum = p.cstate + states * p.N;
+  }
+  return TTT_OK;
+}
+size_t plan_bytes(int rows, int L, int D, int N) {
+  const int n = pieces(rows, L, D, N);
+  if (n <= 1) return 0;
+  const int chunk = piece_tokens(L, n), nchunks = (L + chunk - 1) / chunk;
+  return nchunks > 1 ? (size_t)rows * nchunks * D * (N + 1) * sizeof(float) : 0;
+}
+
+}  // namespace scan
+}  // namespace ttt
+
+using namespace ttt;
+
+extern "C" size_t ttt_selective_scan_fwd_scratch_bytes(int rows, int L, int D, int G, int N) {
+  if (rows < 1 || L < 1 || D < 1 || G < 1 || N < 1 || N > scan::kMaxStates) return 0;
+  return scan::plan_bytes(rows, L, D, N);
+}
+
+extern "C" size_t ttt_selective_scan_saved_bytes(int rows, int L, int D, int N) {
+  if (rows < 1 || L < 1 || D < 1 || N < 1 || N > scan::kMaxStates) return 0;
+  const int every = scan::save_every(N);
+  return (size_t)rows * ((L + every - 1) / every) * D * N * sizeof(float);
+}
+
+extern "C" int ttt_selective_scan_fwd(int rows, int L, int D, int G, int N, const void* u, const void* delta,
+                                      const void* B, const void* C, const void* z, int dt, const long long* strides,
+                                      const float* A, const float* Dskip, const float* delta_bias, int softplus,
+                                      const int* seq, const float* init, float* fin, void* out, float* saved,
+                                      void* scratch, size_t scratch_bytes, void* stream) {
+  const char* who = "ttt_selective_scan_fwd";
+  int rc = scan::check_sizes(who, rows, L, D, G, N, dt);
+  if (rc) return rc;
+  TTT_REQUIRE(u && delta && B && C && A && out && strides, TTT_ERR_NULL, "%s: NULL pointer argument", who);
+  TTT_REQUIRE(!seq || rows == 1, TTT_ERR_SHAPE, "%s: packed sequences lie in one row, got %d", who, rows);
+  scan::Params p{};
+  p.rows = rows, p.L = L, p.D = D, p.G = G, p.N = N, p.Dg = D / G;
+  p.u = u, p.delta = delta, p.B = B, p.C = C, p.z = z;
+  p.u_b = strides[0], p.u_l = strides[1], p.delta_b = strides[2], p.delta_l = strides[3];
+  p.B_b = strides[4], p.B_l = strides[5], p.B_g = strides[6], p.C_b = strides[7], p.C_l = strides[8];
+  p.C_g = strides[9], p.z_b = strides[10], p.z_l = strides[11];
+  p.A = A, p.Dskip = Dskip, p.bias = delta_bias, p.softplus = softplus;
+  p.seq = seq, p.init = init, p.fin = fin, p.out = out, p.hsave = saved;
+  const int every = scan::save_every(N);
+  p.nsave = (L + every - 1) / every;
+  if ((rc = scan::plan(p, scratch, scratch_bytes, 0, who))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (p.nchunks > 1 && (rc = scan::chunk_states(p, dt, false, st, who))) return rc;
+  return dt == DT_BF16  ? scan::launch_fwd<__nv_bfloat16>(p, st, who)
+         : dt == DT_F16 ? scan::launch_fwd<__half>(p, st, who)
+                        : scan::launch_fwd<float>(p, st, who);
+}
+
+extern "C" int ttt_selective_scan_step(int rows, int D, int G, int N, int slots, const void* u, const void* delta,
+                                       const void* B, const void* C, const void* z, int dt, const long long* strides,
+                                       const float* A, const float* Dskip, const float* delta_bias, int softplus,
+                                       const int* index, float* state, void* out, void* stream) {
+  const char* who = "ttt_selective_scan_step";
+  int rc = scan::check_sizes(who, rows, 1, D, G, N, dt);
+  if (rc) return rc;
+  TTT_REQUIRE(u && delta && B && C && A && state && out && strides, TTT_ERR_NULL, "%s: NULL pointer argument", who);
+  TTT_REQUIRE(slots >= 1 && (index || slots >= rows), TTT_ERR_SHAPE, "%s: %d states for %d rows", who, slots, rows);
+  scan::StepParams p{};
+  p.rows = rows, p.D = D, p.G = G, p.N = N, p.Dg = D / G, p.slots = slots;
+  p.u = u, p.delta = delta, p.B = B, p.C = C, p.z = z;
+  p.u_b = strides[0], p.delta_b = strides[1], p.B_b = strides[2], p.B_g = strides[3], p.C_b = strides[4];
+  p.C_g = strides[5], p.z_b = strides[6], p.state_b = strides[7];
+  p.A = A, p.Dskip = Dskip, p.bias = delta_bias, p.softplus = softplus, p.index = index, p.state = state, p.out = out;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return scan::dispatch(N, [&](auto ln, auto npt) {
+    constexpr int LN = decltype(ln)::value, NPT = decltype(npt)::value, DT = 128 / LN;
+    const long long grid = (long long)((D + DT - 1) / DT) * rows;
+    TTT_REQUIRE(grid < (1LL << 31), TTT_ERR_SHAPE, "%s: %lld blocks are too many", who, grid);
+    if (dt == DT_BF16) scan::scan_step_kernel<__nv_bfloat16, LN, NPT><<<(unsigned)grid, 128, 0, st>>>(p);
+    else if (dt == DT_F16) scan::scan_step_kernel<__half, LN, NPT><<<(unsigned)grid, 128, 0, st>>>(p);
+    else scan::scan_step_kernel<float, LN, NPT><<<(unsigned)grid, 128, 0, st>>>(p);
+    return check_launch(who);
+  });
+}
+
+extern "C" int ttt_sequence_index(int T, int S, const int* cu_seqlens, int* seq, void* stream) {
+  const char* who = "ttt_sequence_index";
+  TTT_REQUIRE(cu_seqlens && seq, TTT_ERR_NULL, "%s: NULL pointer argument", who);
+  TTT_REQUIRE(T >= 1 && S >= 1 && T < (1 << 30), TTT_ERR_SHAPE, "%s: bad sizes T=%d S=%d", who, T, S);
+  scan::sequence_index_kernel<<<(T + 255) / 256, 256, 0, static_cast<cudaStream_t>(stream)>>>(T, S, cu_seqlens, seq);
+  return check_launch(who);
+}
