@@ -30,14 +30,29 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + expf(-x)); }
-// log(1 + e^x); above 20 it equals x to less than half an fp32 step.
-__device__ __forceinline__ float softplus(float x) { return x > 20.f ? x : log1pf(expf(x)); }
-// d/dx x sigmoid(x), given sigmoid(x)
-__device__ __forceinline__ float silu_grad(float x, float sg) { return sg * fmaf(x, 1.f - sg, 1.f); }
-
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 1 / (1 + e^-x): two special-function operations, a few steps of 2^-23 off.
+__device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-kLog2e * x)); }
+// log(1 + e^x) = max(x, 0) + log(1 + w), w = e^-|x|, by log(1 + w) = 2 artanh(s), s = w / (2 + w)
+// <= 1/3, and a polynomial in s^2 for 2 artanh(s) / s (least maximum error 8e-9): relative
+// accuracy also where w is small, which a logarithm of 1 + w would lose.
+__device__ __forceinline__ float softplus(float x) {
+  const float w = ex2(-kLog2e * fabsf(x)), s = w * rcp(2.f + w), v = s * s;
+  float q = fmaf(v, 0.2814132571220398f, 0.2797023057937622f);
+  q = fmaf(v, q, 0.4002406597137451f);
+  q = fmaf(v, q, 0.666663408279419f);
+  q = fmaf(v, q, 2.f);
+  return fmaf(s, q, fmaxf(x, 0.f));
+}
+// d/dx x sigmoid(x), given sigmoid(x)
+__device__ __forceinline__ float silu_grad(float x, float sg) { return sg * fmaf(x, 1.f - sg, 1.f); }
 
 // Packed rows: seq[t] is the sequence that token t belongs to, -1 for tokens of none. A token
 // whose predecessor belongs to another sequence starts its own, and likewise at the end.

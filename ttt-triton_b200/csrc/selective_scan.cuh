@@ -25,6 +25,7 @@ struct Params {
   long long u_b, u_l, delta_b, delta_l, B_b, B_l, B_g, C_b, C_l, C_g, z_b, z_l;  // element strides
   const float *A, *Dskip, *bias;
   int softplus;
+  int quads;           // rows of B and C are read four states at a time
   const int* seq;      // packed rows: each token's sequence (rows == 1), else NULL
   const float* init;   // [sequences, D, N] or NULL
   float* fin;          // [sequences, D, N] or NULL
@@ -59,34 +60,137 @@ inline int save_every(int N) { return 64 / shape_of(N).NPT; }
 
 __device__ __forceinline__ float step_size(const Params& p, float raw) { return p.softplus ? softplus(raw) : raw; }
 
-// Loads this thread's NPT states of channel d from a [.., D, N] array (0 past N).
+// This thread's NPT states of channel d of a [.., D, N] array (0 past N); in fours where N is a
+// multiple of four and the array lies on a 16-byte boundary, as torch's allocations do.
 template <int NPT>
 __device__ __forceinline__ void load_states(const float* base, int d, int n0, int N, bool on, float (&h)[NPT]) {
+  const float* p = base + (long long)d * N + n0;
+  if (N % 4 == 0 && (reinterpret_cast<uintptr_t>(base) & 15) == 0) {
 #pragma unroll
-  for (int i = 0; i < NPT; ++i) h[i] = on && n0 + i < N ? base[(long long)d * N + n0 + i] : 0.f;
+    for (int i = 0; i < NPT; i += 4) {
+      float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (on && n0 + i < N) q = *reinterpret_cast<const float4*>(p + i);
+      h[i] = q.x, h[i + 1] = q.y, h[i + 2] = q.z, h[i + 3] = q.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < NPT; ++i) h[i] = on && n0 + i < N ? p[i] : 0.f;
 }
 template <int NPT>
 __device__ __forceinline__ void store_states(float* base, int d, int n0, int N, bool on, const float (&h)[NPT]) {
+  float* p = base + (long long)d * N + n0;
+  if (N % 4 == 0 && (reinterpret_cast<uintptr_t>(base) & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < NPT; i += 4)
+      if (on && n0 + i < N) *reinterpret_cast<float4*>(p + i) = make_float4(h[i], h[i + 1], h[i + 2], h[i + 3]);
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < NPT; ++i)
-    if (on && n0 + i < N) base[(long long)d * N + n0 + i] = h[i];
+    if (on && n0 + i < N) p[i] = h[i];
 }
 
 // Stages rows t0 .. t0 + TT - 1 of B or C as fp32 in shared memory (0 past the end, past N and
-// for tokens of no sequence).
+// for tokens of no sequence). `quads`: four states at a time, where every row is N = NP states
+// on a boundary of four.
 template <typename T, int NP, int TT, int THREADS>
 __device__ __forceinline__ void stage_rows(float* dst, const T* src, long long ld, int t0, int t1, int N,
-                                           const int* seq) {
+                                           const int* seq, bool quads) {
+  if (quads) {
+    struct alignas(4 * sizeof(T)) Quad {
+      T v[4];
+    };
+#pragma unroll
+    for (int k = 0; k < (TT * NP / 4 + THREADS - 1) / THREADS; ++k) {
+      const int i = threadIdx.x + k * THREADS, t = i / (NP / 4), n = i % (NP / 4) * 4;
+      if (TT * NP / 4 % THREADS == 0 || i < TT * NP / 4) {
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (t0 + t < t1 && !(seq && seq[t0 + t] < 0)) {
+          const Quad q = *reinterpret_cast<const Quad*>(src + (t0 + t) * ld + n);
+          f = make_float4(to_f(q.v[0]), to_f(q.v[1]), to_f(q.v[2]), to_f(q.v[3]));
+        }
+        *reinterpret_cast<float4*>(dst + i * 4) = f;
+      }
+    }
+    return;
+  }
   for (int i = threadIdx.x; i < TT * NP; i += THREADS) {
     const int t = i / NP, n = i - t * NP;
     dst[i] = t0 + t < t1 && n < N && !(seq && seq[t0 + t] < 0) ? to_f(src[(t0 + t) * ld + n]) : 0.f;
   }
 }
 
+// NPT states as pairs, and a tile row's values for them.
+template <int NPT>
+struct Pairs {
+  float2 v[NPT / 2];
+};
+template <int NPT>
+__device__ __forceinline__ Pairs<NPT> pairs_of(const float (&x)[NPT]) {
+  Pairs<NPT> r;
+#pragma unroll
+  for (int j = 0; j < NPT / 2; ++j) r.v[j] = make_float2(x[2 * j], x[2 * j + 1]);
+  return r;
+}
+template <int NPT>
+__device__ __forceinline__ void unpair(const Pairs<NPT>& x, float (&y)[NPT]) {
+#pragma unroll
+  for (int j = 0; j < NPT / 2; ++j) y[2 * j] = x.v[j].x, y[2 * j + 1] = x.v[j].y;
+}
+template <int NPT>
+__device__ __forceinline__ Pairs<NPT> row_pairs(const float* row) {  // 16-byte aligned
+  Pairs<NPT> r;
+#pragma unroll
+  for (int j = 0; j < NPT / 4; ++j) {
+    const float4 q = reinterpret_cast<const float4*>(row)[j];
+    r.v[2 * j] = make_float2(q.x, q.y), r.v[2 * j + 1] = make_float2(q.z, q.w);
+  }
+  return r;
+}
+
+// 2^x for the products x = dt A2 of a pair of states. The special-function unit gives 16 an SM
+// and clock, the fused multiply-add pipes stand half idle beside it, so a part of the pairs
+// goes there: x = k + f, 2^f = 1 + f q(f) with q of degree 4 (relative error 1.2e-7, and that
+// of a rounding near 1, where decays act longest), k into the exponent. That form holds for
+// |x| < 126 only; kernels look at a tile's largest |dt| times the largest |A2| first.
+constexpr float kPolyRange = 126.f;
+__device__ __forceinline__ float2 pow2_poly(float2 dt, float2 A2) {
+  const float2 magic = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23: the sum's low bits are k
+  const float2 xi = __ffma2_rn(dt, A2, magic);
+  const float2 k = __fadd2_rn(xi, make_float2(-12582912.f, -12582912.f));
+  const float2 f = __ffma2_rn(dt, A2, make_float2(-k.x, -k.y));
+  float2 q = __ffma2_rn(f, make_float2(0.0013405575882643461f, 0.0013405575882643461f),
+                        make_float2(0.009670727886259556f, 0.009670727886259556f));
+  q = __ffma2_rn(f, q, make_float2(0.05550314858555794f, 0.05550314858555794f));
+  q = __ffma2_rn(f, q, make_float2(0.24022258818149567f, 0.24022258818149567f));
+  q = __ffma2_rn(f, q, make_float2(0.6931471824645996f, 0.6931471824645996f));
+  q = __ffma2_rn(f, q, make_float2(1.f, 1.f));
+  return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(xi.x) << 23)),
+                     __int_as_float(__float_as_int(q.y) + (__float_as_int(xi.y) << 23)));
+}
+__device__ __forceinline__ float2 pow2_unit(float2 dt, float2 A2) {
+  const float2 x = __fmul2_rn(dt, A2);
+  return make_float2(ex2(x.x), ex2(x.y));
+}
+
+// The largest |x| of a CTA as integer bits (NaN above all): per warp, for a tile's readers.
+__device__ __forceinline__ unsigned warp_max_abs(float x) {
+  return __reduce_max_sync(0xffffffffu, __float_as_uint(x) & 0x7fffffffu);
+}
+template <int WARPS>
+__device__ __forceinline__ float max_of(const unsigned (&m)[WARPS]) {
+  unsigned v = m[0];
+#pragma unroll
+  for (int k = 1; k < WARPS; ++k) v = max(v, m[k]);
+  return __uint_as_float(v);
+}
+
 // Start, end and membership of the tile's tokens as bit masks (at most 32 tokens).
 struct SeqMask {
   unsigned start, end, in;
 };
+__device__ __forceinline__ bool in_sequence(const int* seq, int t) { return !seq || seq[t] >= 0; }
 template <int TT>
 __device__ __forceinline__ void stage_masks(SeqMask* m, const int* seq, int t0, int t1, int T) {
   if (threadIdx.x < 32) {
@@ -104,6 +208,7 @@ __device__ __forceinline__ void stage_masks(SeqMask* m, const int* seq, int t0, 
 int chunk_states(const Params& p, int dt, bool rev, cudaStream_t st, const char* who);
 // Splits the time axis and lays its part of the scratch out behind `extra` bytes of the caller.
 int plan(Params& p, void* scratch, size_t scratch_bytes, size_t extra, const char* who);
+bool quads(const Params& p, int dt);
 size_t plan_bytes(int rows, int L, int D, int N);
 int check_sizes(const char* who, int rows, int L, int D, int G, int N, int dt);
 

@@ -18,140 +18,233 @@ namespace scan {
 
 template <int LN, int NPT>
 struct Fwd {
-  static constexpr int THREADS = 128;
+  static constexpr int THREADS = 128, WARPS = THREADS / 32;
   static constexpr int DT = THREADS / LN;            // channels of a CTA
   static constexpr int NP = LN * NPT;                // states, padded
   static constexpr int TT = LN >= 4 ? 32 : 8 * LN;   // tokens of a tile
+  static constexpr int RUN = 8;                      // tokens unrolled
   static constexpr int PAIRS = TT * DT / THREADS;    // (token, channel) pairs of a thread
   struct Smem {
     float B[TT * NP], C[TT * NP];
-    float2 d[TT * DT];      // step size, step size * input
+    float4 d[TT * DT];      // step size twice, step size * input twice: operands of paired arithmetic
     float y[TT * THREADS];  // partial outputs
+    unsigned dt_max[WARPS], A_max[WARPS];
     SeqMask m;
   };
 };
 
-template <typename T, int LN, int NPT>
+// What a thread holds: channel d and states n0 .. in the recurrence; channel pd, and tokens
+// tq, tq + LN, .. of a tile, in the element-wise passes.
+template <int LN, int NPT>
+struct Lane {
+  int n0, cl, d, tq, pc, pd;
+  bool on, pon;
+  __device__ __forceinline__ Lane(const Params& p, const Where& w) {
+    using F = Fwd<LN, NPT>;
+    const int tid = threadIdx.x;
+    n0 = tid % LN * NPT, cl = tid / LN;
+    pc = tid % F::DT, tq = tid / F::DT;
+    d = w.g * p.Dg + w.d0 + cl, pd = w.g * p.Dg + w.d0 + pc;
+    on = w.d0 + cl < p.Dg, pon = w.d0 + pc < p.Dg;
+  }
+};
+
+// One token of the recurrence for NPT states; POLY: this token's share of the decays goes to
+// the multiply-add pipes (3 pairs in 8, see pow2_poly).
+template <int NPT, bool POLY>
+__device__ __forceinline__ void advance(Pairs<NPT>& h, const Pairs<NPT>& A2, const float4 dd, const float* Brow,
+                                        int t) {
+  const float2 dt = make_float2(dd.x, dd.y), dtu = make_float2(dd.z, dd.w);
+  const Pairs<NPT> B = row_pairs<NPT>(Brow);
+#pragma unroll
+  for (int j = 0; j < NPT / 2; ++j) {
+    const int k = (t * (NPT / 2) + j) % 8;
+    const float2 a = POLY && (k == 1 || k == 4 || k == 6) ? pow2_poly(dt, A2.v[j]) : pow2_unit(dt, A2.v[j]);
+    h.v[j] = __ffma2_rn(a, h.v[j], __fmul2_rn(dtu, B.v[j]));
+  }
+}
+
+template <typename T, int LN, int NPT, bool SEQ>
 __global__ void __launch_bounds__(128) scan_fwd_kernel(const __grid_constant__ Params p) {
   using F = Fwd<LN, NPT>;
   extern __shared__ __align__(16) unsigned char raw_smem[];
   auto& s = *reinterpret_cast<typename F::Smem*>(raw_smem);
   const Where w = where<F::DT>(p);
-  const int tid = threadIdx.x, nl = tid % LN, cl = tid / LN;
-  const int n0 = nl * NPT;
-  const int d = w.g * p.Dg + w.d0 + cl;              // this thread's channel in the recurrence
-  const bool on = w.d0 + cl < p.Dg;
-  const int pc = tid % F::DT, pd = w.g * p.Dg + w.d0 + pc;  // and in the element-wise passes
-  const bool pon = w.d0 + pc < p.Dg;
+  const Lane<LN, NPT> q(p, w);
+  const int tid = threadIdx.x;
   const int tbeg = w.piece * p.chunk, tend = min(p.L, tbeg + p.chunk);
+  const long long DN = (long long)p.D * p.N;
+  const int* seq = SEQ ? p.seq : nullptr;
 
-  float A2[NPT], h[NPT];
-  load_states<NPT>(p.A, d, n0, p.N, on, A2);
+  float hs[NPT];
+  load_states<NPT>(p.A, q.d, q.n0, p.N, q.on, hs);
+  float amax = 0.f;
 #pragma unroll
-  for (int i = 0; i < NPT; ++i) A2[i] *= kLog2e;
+  for (int i = 0; i < NPT; ++i) {
+    hs[i] *= kLog2e;
+    amax = fabsf(hs[i]) <= amax ? amax : fabsf(hs[i]);  // a NaN stays
+  }
+  const unsigned am = warp_max_abs(amax);
+  if (tid % 32 == 0) s.A_max[tid / 32] = am;
+  const Pairs<NPT> A2 = pairs_of<NPT>(hs);
   if (p.nchunks > 1)
-    load_states<NPT>(p.cstate + ((long long)w.row * p.nchunks + w.piece) * p.D * p.N, d, n0, p.N, on, h);
-  else if (p.init && !p.seq)
-    load_states<NPT>(p.init + (long long)w.row * p.D * p.N, d, n0, p.N, on, h);
+    load_states<NPT>(p.cstate + ((long long)w.row * p.nchunks + w.piece) * DN, q.d, q.n0, p.N, q.on, hs);
   else
-    load_states<NPT>(p.A, d, n0, p.N, false, h);
-  const float skip = pon && p.Dskip ? p.Dskip[pd] : 0.f, bias = pon && p.bias ? p.bias[pd] : 0.f;
-  const T* u = static_cast<const T*>(p.u) + w.row * p.u_b + pd;
-  const T* delta = static_cast<const T*>(p.delta) + w.row * p.delta_b + pd;
-  const T* z = p.z ? static_cast<const T*>(p.z) + w.row * p.z_b + pd : nullptr;
+    load_states<NPT>(p.init + w.row * DN, q.d, q.n0, p.N, q.on && p.init && !SEQ, hs);
+  Pairs<NPT> h = pairs_of<NPT>(hs);
+  const float skip = q.pon && p.Dskip ? p.Dskip[q.pd] : 0.f, bias = q.pon && p.bias ? p.bias[q.pd] : 0.f;
+  const long long first = tbeg + q.tq;
+  const T* u = static_cast<const T*>(p.u) + w.row * p.u_b + first * p.u_l + q.pd;
+  const T* delta = static_cast<const T*>(p.delta) + w.row * p.delta_b + first * p.delta_l + q.pd;
+  const T* z = p.z ? static_cast<const T*>(p.z) + w.row * p.z_b + first * p.z_l + q.pd : nullptr;
   const T* B = static_cast<const T*>(p.B) + w.row * p.B_b + w.g * p.B_g;
   const T* C = static_cast<const T*>(p.C) + w.row * p.C_b + w.g * p.C_g;
-  T* out = static_cast<T*>(p.out) + (long long)w.row * p.L * p.D + pd;
+  T* out = static_cast<T*>(p.out) + ((long long)w.row * p.L + first) * p.D + q.pd;
   const int every = 64 / NPT;
 
   for (int t0 = tbeg; t0 < tend; t0 += F::TT) {
-    float uu[F::PAIRS], zz[F::PAIRS];
-    if (p.seq) stage_masks<F::TT>(&s.m, p.seq, t0, tend, p.L);
+    T uu[F::PAIRS], zz[F::PAIRS], dd[F::PAIRS];
+    if (SEQ) stage_masks<F::TT>(&s.m, p.seq, t0, tend, p.L);
 #pragma unroll
     for (int k = 0; k < F::PAIRS; ++k) {
-      const int t = tid / F::DT + k * LN, tok = t0 + t;
-      float dt = 0.f;
-      uu[k] = zz[k] = 0.f;
-      if (pon && tok < tend && !(p.seq && p.seq[tok] < 0)) {
-        uu[k] = to_f(u[tok * p.u_l]);
-        dt = step_size(p, to_f(delta[tok * p.delta_l]) + bias);
-        if (z) zz[k] = to_f(z[tok * p.z_l]);
+      const int tok = t0 + q.tq + k * LN;
+      const bool on = q.pon && tok < tend && in_sequence(seq, tok);
+      dd[k] = from_f<T>(0.f), uu[k] = zz[k] = dd[k];
+      if (on) {
+        dd[k] = delta[k * LN * p.delta_l], uu[k] = u[k * LN * p.u_l];
+        if (z) zz[k] = z[k * LN * p.z_l];
       }
-      s.d[t * F::DT + pc] = make_float2(dt, dt * uu[k]);
     }
-    stage_rows<T, F::NP, F::TT, F::THREADS>(s.B, B, p.B_l, t0, tend, p.N, p.seq);
-    stage_rows<T, F::NP, F::TT, F::THREADS>(s.C, C, p.C_l, t0, tend, p.N, p.seq);
-    __syncthreads();
-
-    for (int t = 0; t < F::TT; ++t) {
-      if (t0 + t >= tend) break;
-      if (p.hsave && (t0 + t) % every == 0)
-        store_states<NPT>(p.hsave + ((long long)w.row * p.nsave + (t0 + t) / every) * p.D * p.N, d, n0, p.N, on, h);
-      if (p.seq && (s.m.start >> t & 1)) {
-        const int q = p.seq[t0 + t];
-        load_states<NPT>(p.init + (long long)q * p.D * p.N, d, n0, p.N, on && q >= 0 && p.init, h);
-      }
-      const float2 dd = s.d[t * F::DT + cl];
-      float y = 0.f;
+    stage_rows<T, F::NP, F::TT, F::THREADS>(s.B, B, p.B_l, t0, tend, p.N, seq, p.quads);
+    stage_rows<T, F::NP, F::TT, F::THREADS>(s.C, C, p.C_l, t0, tend, p.N, seq, p.quads);
+    float m = 0.f;
 #pragma unroll
-      for (int i = 0; i < NPT; ++i) {
-        h[i] = fmaf(ex2(dd.x * A2[i]), h[i], dd.y * s.B[t * F::NP + n0 + i]);
-        y = fmaf(h[i], s.C[t * F::NP + n0 + i], y);
+    for (int k = 0; k < F::PAIRS; ++k) {
+      const int tok = t0 + q.tq + k * LN;
+      const bool on = q.pon && tok < tend && in_sequence(seq, tok);
+      const float dt = on ? step_size(p, to_f(dd[k]) + bias) : 0.f, x = dt * to_f(uu[k]);
+      m = fabsf(dt) <= m ? m : fabsf(dt);
+      s.d[(q.tq + k * LN) * F::DT + q.pc] = make_float4(dt, dt, x, x);
+    }
+    const unsigned wm = warp_max_abs(m);
+    if (tid % 32 == 0) s.dt_max[tid / 32] = wm;
+    __syncthreads();
+    const bool poly = max_of(s.dt_max) * max_of(s.A_max) < kPolyRange;
+
+#pragma unroll 1
+    for (int r = 0; r < F::TT && t0 + r < tend; r += F::RUN) {
+      if (p.hsave && (t0 + r) % every == 0) {
+        unpair(h, hs);
+        store_states<NPT>(p.hsave + ((long long)w.row * p.nsave + (t0 + r) / every) * DN, q.d, q.n0, p.N, q.on, hs);
       }
-      s.y[t * F::THREADS + tid] = y;
-      if (p.seq && p.fin && (s.m.end >> t & 1)) {
-        const int q = p.seq[t0 + t];
-        store_states<NPT>(p.fin + (long long)q * p.D * p.N, d, n0, p.N, on && q >= 0, h);
-      }
+      const bool slow =
+          t0 + r + F::RUN > tend || (SEQ && ((s.m.start | s.m.end) >> r & 0xff)) || (p.hsave && every < F::RUN);
+      const auto tokens = [&](auto use_poly, auto checks) {
+#pragma unroll
+        for (int k = 0; k < F::RUN; ++k) {
+          const int t = r + k;
+          if constexpr (decltype(checks)::value) {
+            if (t0 + t >= tend) break;
+            if (p.hsave && k && (t0 + t) % every == 0) {
+              unpair(h, hs);
+              store_states<NPT>(p.hsave + ((long long)w.row * p.nsave + (t0 + t) / every) * DN, q.d, q.n0, p.N, q.on,
+                                hs);
+            }
+            if (SEQ && (s.m.start >> t & 1)) {
+              const int sq = p.seq[t0 + t];
+              load_states<NPT>(p.init + sq * DN, q.d, q.n0, p.N, q.on && sq >= 0 && p.init, hs);
+              h = pairs_of<NPT>(hs);
+            }
+          }
+          advance<NPT, decltype(use_poly)::value>(h, A2, s.d[t * F::DT + q.cl], s.B + t * F::NP + q.n0, k);
+          const Pairs<NPT> C2 = row_pairs<NPT>(s.C + t * F::NP + q.n0);
+          float2 y = __fmul2_rn(h.v[0], C2.v[0]);
+#pragma unroll
+          for (int j = 1; j < NPT / 2; ++j) y = __ffma2_rn(h.v[j], C2.v[j], y);
+          s.y[t * F::THREADS + tid] = y.x + y.y;
+          if constexpr (decltype(checks)::value) {
+            if (SEQ && p.fin && (s.m.end >> t & 1)) {
+              const int sq = p.seq[t0 + t];
+              unpair(h, hs);
+              store_states<NPT>(p.fin + sq * DN, q.d, q.n0, p.N, q.on && sq >= 0, hs);
+            }
+          }
+        }
+      };
+      if (slow) tokens(std::false_type{}, std::true_type{});
+      else if (poly) tokens(std::true_type{}, std::false_type{});
+      else tokens(std::false_type{}, std::false_type{});
     }
     __syncthreads();
 
 #pragma unroll
     for (int k = 0; k < F::PAIRS; ++k) {
-      const int t = tid / F::DT + k * LN, tok = t0 + t;
-      if (pon && tok < tend) {
+      const int t = q.tq + k * LN, tok = t0 + t;
+      if (q.pon && tok < tend) {
         float y = 0.f;
+        if constexpr (LN >= 4) {
 #pragma unroll
-        for (int j = 0; j < LN; ++j) y += s.y[t * F::THREADS + pc * LN + j];
-        y = fmaf(skip, uu[k], y);
-        if (z) y *= zz[k] * sigmoid(zz[k]);
-        if (p.seq && !(s.m.in >> t & 1)) y = 0.f;  // a token of no sequence
-        out[(long long)tok * p.D] = from_f<T>(y);
+          for (int j = 0; j < LN / 4; ++j) {
+            const float4 v = reinterpret_cast<const float4*>(s.y + t * F::THREADS + q.pc * LN)[j];
+            y += (v.x + v.y) + (v.z + v.w);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < LN; ++j) y += s.y[t * F::THREADS + q.pc * LN + j];
+        }
+        y = fmaf(skip, to_f(uu[k]), y);
+        if (z) {
+          const float g = to_f(zz[k]);
+          y *= g * sigmoid(g);
+        }
+        if (SEQ && !(s.m.in >> t & 1)) y = 0.f;  // a token of no sequence
+        out[(long long)k * LN * p.D] = from_f<T>(y);
       }
     }
-    if (p.seq) __syncthreads();  // the masks are written again
+    u += F::TT * p.u_l, delta += F::TT * p.delta_l, out += (long long)F::TT * p.D;
+    if (z) z += F::TT * p.z_l;
+    if (SEQ) __syncthreads();  // the masks are written again
   }
-  if (!p.seq && p.fin && tend == p.L)
-    store_states<NPT>(p.fin + (long long)w.row * p.D * p.N, d, n0, p.N, on, h);
+  if (!SEQ && p.fin && tend == p.L) {
+    unpair(h, hs);
+    store_states<NPT>(p.fin + w.row * DN, q.d, q.n0, p.N, q.on, hs);
+  }
 }
 
 // A piece's end state from zero (REV: the carry that leaves its first token from zero at its
 // last), and the sum of its step sizes.
-template <typename T, int LN, int NPT, bool REV>
+template <typename T, int LN, int NPT, bool REV, bool SEQ>
 __global__ void __launch_bounds__(128) scan_chunk_kernel(const __grid_constant__ Params p) {
   using F = Fwd<LN, NPT>;
   extern __shared__ __align__(16) unsigned char raw_smem[];
   auto& s = *reinterpret_cast<typename F::Smem*>(raw_smem);
   const Where w = where<F::DT>(p);
-  const int tid = threadIdx.x, nl = tid % LN, cl = tid / LN;
-  const int n0 = nl * NPT;
-  const int d = w.g * p.Dg + w.d0 + cl;
-  const bool on = w.d0 + cl < p.Dg;
-  const int pc = tid % F::DT, pd = w.g * p.Dg + w.d0 + pc;
-  const bool pon = w.d0 + pc < p.Dg;
+  const Lane<LN, NPT> q(p, w);
+  const int tid = threadIdx.x;
   const int tbeg = w.piece * p.chunk, tend = min(p.L, tbeg + p.chunk);
+  const long long DN = (long long)p.D * p.N;
+  const int* seq = SEQ ? p.seq : nullptr;
 
-  float A2[NPT], h[NPT], sum = 0.f;
-  load_states<NPT>(p.A, d, n0, p.N, on, A2);
+  float hs[NPT], sum = 0.f, amax = 0.f;
+  load_states<NPT>(p.A, q.d, q.n0, p.N, q.on, hs);
 #pragma unroll
-  for (int i = 0; i < NPT; ++i) A2[i] *= kLog2e, h[i] = 0.f;
-  const float bias = pon && p.bias ? p.bias[pd] : 0.f;
-  const T* delta = static_cast<const T*>(p.delta) + w.row * p.delta_b + pd;
+  for (int i = 0; i < NPT; ++i) {
+    hs[i] *= kLog2e;
+    amax = fabsf(hs[i]) <= amax ? amax : fabsf(hs[i]);
+  }
+  const unsigned am = warp_max_abs(amax);
+  if (tid % 32 == 0) s.A_max[tid / 32] = am;
+  const Pairs<NPT> A2 = pairs_of<NPT>(hs);
+  Pairs<NPT> h;
+#pragma unroll
+  for (int j = 0; j < NPT / 2; ++j) h.v[j] = make_float2(0.f, 0.f);
+  const float bias = q.pon && p.bias ? p.bias[q.pd] : 0.f;
+  const T* delta = static_cast<const T*>(p.delta) + w.row * p.delta_b + q.pd;
   // what drives the recurrence: u and B, or dout (gated) and C
-  const T* v = REV ? static_cast<const T*>(p.dout) + (long long)w.row * p.L * p.D + pd
-                   : static_cast<const T*>(p.u) + w.row * p.u_b + pd;
+  const T* v = REV ? static_cast<const T*>(p.dout) + (long long)w.row * p.L * p.D + q.pd
+                   : static_cast<const T*>(p.u) + w.row * p.u_b + q.pd;
   const long long v_l = REV ? p.D : p.u_l;
-  const T* z = REV && p.z ? static_cast<const T*>(p.z) + w.row * p.z_b + pd : nullptr;
+  const T* z = REV && p.z ? static_cast<const T*>(p.z) + w.row * p.z_b + q.pd : nullptr;
   const T* R = REV ? static_cast<const T*>(p.C) + w.row * p.C_b + w.g * p.C_g
                    : static_cast<const T*>(p.B) + w.row * p.B_b + w.g * p.B_g;
   const long long r_l = REV ? p.C_l : p.B_l;
@@ -160,44 +253,83 @@ __global__ void __launch_bounds__(128) scan_chunk_kernel(const __grid_constant__
   const int ntiles = (tend - tbeg + F::TT - 1) / F::TT;
   for (int k0 = 0; k0 < ntiles; ++k0) {
     const int t0 = tbeg + (REV ? ntiles - 1 - k0 : k0) * F::TT;
-    if (p.seq) stage_masks<F::TT>(&s.m, p.seq, t0, tend, p.L);
+    if (SEQ) stage_masks<F::TT>(&s.m, p.seq, t0, tend, p.L);
+    T dd[F::PAIRS], vv[F::PAIRS], zz[F::PAIRS];
 #pragma unroll
     for (int k = 0; k < F::PAIRS; ++k) {
-      const int t = tid / F::DT + k * LN, tok = t0 + t;
-      float dt = 0.f, x = 0.f;
-      if (pon && tok < tend && !(p.seq && p.seq[tok] < 0)) {
-        dt = step_size(p, to_f(delta[tok * p.delta_l]) + bias);
-        x = to_f(v[tok * v_l]);
-        if (REV && z) {
-          const float zz = to_f(z[tok * p.z_l]);
-          x *= zz * sigmoid(zz);
-        }
-        if (!REV) x *= dt;
+      const int tok = t0 + q.tq + k * LN;
+      const bool on = q.pon && tok < tend && in_sequence(seq, tok);
+      dd[k] = from_f<T>(0.f), vv[k] = zz[k] = dd[k];
+      if (on) {
+        dd[k] = delta[tok * p.delta_l], vv[k] = v[tok * v_l];
+        if (REV && z) zz[k] = z[tok * p.z_l];
       }
-      s.d[t * F::DT + pc] = make_float2(dt, x);
     }
-    stage_rows<T, F::NP, F::TT, F::THREADS>(s.B, R, r_l, t0, tend, p.N, p.seq);
-    __syncthreads();
-    for (int k = 0; k < F::TT; ++k) {
-      const int t = REV ? F::TT - 1 - k : k;
-      if (t0 + t >= tend) continue;
-      if (p.seq && ((REV ? s.m.end : s.m.start) >> t & 1)) {
-        const int q = p.seq[t0 + t];
-        load_states<NPT>(edge + (long long)q * p.D * p.N, d, n0, p.N, on && q >= 0 && edge, h);
-      }
-      const float2 dd = s.d[t * F::DT + cl];
-      sum += dd.x;
+    stage_rows<T, F::NP, F::TT, F::THREADS>(s.B, R, r_l, t0, tend, p.N, seq, p.quads);
+    float m = 0.f;
 #pragma unroll
-      for (int i = 0; i < NPT; ++i) {
-        const float a = ex2(dd.x * A2[i]), x = dd.y * s.B[t * F::NP + n0 + i];
-        h[i] = REV ? a * (h[i] + x) : fmaf(a, h[i], x);
+    for (int k = 0; k < F::PAIRS; ++k) {
+      const int tok = t0 + q.tq + k * LN;
+      const bool on = q.pon && tok < tend && in_sequence(seq, tok);
+      const float dt = on ? step_size(p, to_f(dd[k]) + bias) : 0.f;
+      float x = to_f(vv[k]);
+      if (REV && z) {
+        const float g = to_f(zz[k]);
+        x *= g * sigmoid(g);
       }
+      if (!REV) x *= dt;
+      m = fabsf(dt) <= m ? m : fabsf(dt);
+      s.d[(q.tq + k * LN) * F::DT + q.pc] = make_float4(dt, dt, x, x);
+    }
+    const unsigned wm = warp_max_abs(m);
+    if (tid % 32 == 0) s.dt_max[tid / 32] = wm;
+    __syncthreads();
+    const bool poly = max_of(s.dt_max) * max_of(s.A_max) < kPolyRange;
+
+#pragma unroll 1
+    for (int r0 = 0; r0 < F::TT; r0 += F::RUN) {
+      const int r = REV ? F::TT - F::RUN - r0 : r0;
+      if (t0 + r >= tend) continue;
+      const auto tokens = [&](auto use_poly, auto checks) {
+#pragma unroll
+        for (int k = 0; k < F::RUN; ++k) {
+          const int t = r + (REV ? F::RUN - 1 - k : k);
+          if constexpr (decltype(checks)::value) {
+            if (t0 + t >= tend) continue;
+            if (SEQ && ((REV ? s.m.end : s.m.start) >> t & 1)) {
+              const int sq = p.seq[t0 + t];
+              load_states<NPT>(edge + sq * DN, q.d, q.n0, p.N, q.on && sq >= 0 && edge, hs);
+              h = pairs_of<NPT>(hs);
+            }
+          }
+          const float4 dd4 = s.d[t * F::DT + q.cl];
+          const float* row = s.B + t * F::NP + q.n0;
+          sum += dd4.x;
+          if constexpr (REV) {
+            const Pairs<NPT> R2 = row_pairs<NPT>(row);
+            const float2 dt = make_float2(dd4.x, dd4.y), x = make_float2(dd4.z, dd4.w);
+#pragma unroll
+            for (int j = 0; j < NPT / 2; ++j) {
+              const int i = (k * (NPT / 2) + j) % 8;
+              const float2 a = decltype(use_poly)::value && (i == 1 || i == 4 || i == 6) ? pow2_poly(dt, A2.v[j])
+                                                                                         : pow2_unit(dt, A2.v[j]);
+              h.v[j] = __fmul2_rn(a, __ffma2_rn(x, R2.v[j], h.v[j]));
+            }
+          } else {
+            advance<NPT, decltype(use_poly)::value>(h, A2, dd4, row, k);
+          }
+        }
+      };
+      if (t0 + r + F::RUN > tend || (SEQ && ((REV ? s.m.end : s.m.start) >> r & 0xff))) tokens(std::false_type{}, std::true_type{});
+      else if (poly) tokens(std::true_type{}, std::false_type{});
+      else tokens(std::false_type{}, std::false_type{});
     }
     __syncthreads();
   }
   const long long at = (long long)w.row * p.nchunks + w.piece;
-  store_states<NPT>(p.cstate + at * p.D * p.N, d, n0, p.N, on, h);
-  if (on && nl == 0) p.csum[at * p.D + d] = sum;
+  unpair(h, hs);
+  store_states<NPT>(p.cstate + at * DN, q.d, q.n0, p.N, q.on, hs);
+  if (q.on && tid % LN == 0) p.csum[at * p.D + q.d] = sum;
 }
 
 // Turns the pieces' end states into the states that enter them, in place. One thread per
@@ -301,7 +433,8 @@ template <typename T>
 static int launch_fwd(Params p, cudaStream_t st, const char* who) {
   return dispatch(p.N, [&](auto ln, auto npt) {
     using F = Fwd<decltype(ln)::value, decltype(npt)::value>;
-    auto kernel = scan_fwd_kernel<T, decltype(ln)::value, decltype(npt)::value>;
+    constexpr int LN = decltype(ln)::value, NPT = decltype(npt)::value;
+    auto kernel = p.seq ? scan_fwd_kernel<T, LN, NPT, true> : scan_fwd_kernel<T, LN, NPT, false>;
     Params q = p;
     q.tiles = (p.Dg + F::DT - 1) / F::DT;
     const int rc = prepare_smem(kernel, sizeof(typename F::Smem), who);
@@ -317,7 +450,8 @@ template <typename T, bool REV>
 static int launch_chunks(Params p, cudaStream_t st, const char* who) {
   return dispatch(p.N, [&](auto ln, auto npt) {
     using F = Fwd<decltype(ln)::value, decltype(npt)::value>;
-    auto kernel = scan_chunk_kernel<T, decltype(ln)::value, decltype(npt)::value, REV>;
+    constexpr int LN = decltype(ln)::value, NPT = decltype(npt)::value;
+    auto kernel = p.seq ? scan_chunk_kernel<T, LN, NPT, REV, true> : scan_chunk_kernel<T, LN, NPT, REV, false>;
     Params q = p;
     q.tiles = (p.Dg + F::DT - 1) / F::DT;
     int rc = prepare_smem(kernel, sizeof(typename F::Smem), who);
@@ -339,6 +473,16 @@ int chunk_states(const Params& p, int dt, bool rev, cudaStream_t st, const char*
   return dt == DT_BF16  ? launch_chunks<__nv_bfloat16, false>(p, st, who)
          : dt == DT_F16 ? launch_chunks<__half, false>(p, st, who)
                         : launch_chunks<float, false>(p, st, who);
+}
+
+// Whether stage_rows may read B and C four states at a time.
+bool quads(const Params& p, int dt) {
+  const int elem = dt == DT_F32 ? 4 : 2;
+  const Shape s = shape_of(p.N);
+  if (p.N != s.LN * s.NPT) return false;
+  for (const long long st : {p.B_b, p.B_l, p.B_g, p.C_b, p.C_l, p.C_g})
+    if (st % 4) return false;
+  return reinterpret_cast<uintptr_t>(p.B) % (4 * elem) == 0 && reinterpret_cast<uintptr_t>(p.C) % (4 * elem) == 0;
 }
 
 // Pieces of the time axis: as many as bring the device about two full waves of warps, no
@@ -424,6 +568,7 @@ extern "C" int ttt_selective_scan_fwd(int rows, int L, int D, int G, int N, cons
   p.seq = seq, p.init = init, p.fin = fin, p.out = out, p.hsave = saved;
   const int every = scan::save_every(N);
   p.nsave = (L + every - 1) / every;
+  p.quads = scan::quads(p, dt);
   if ((rc = scan::plan(p, scratch, scratch_bytes, 0, who))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (p.nchunks > 1 && (rc = scan::chunk_states(p, dt, false, st, who))) return rc;

@@ -92,8 +92,8 @@ __global__ void __launch_bounds__(256) scan_bwd_kernel(const __grid_constant__ P
         s.dt[t * F::DT + pc] = dt, s.dtu[t * F::DT + pc] = dt * uu[k], s.dy[t * F::DT + pc] = dy;
       }
     }
-    stage_rows<T, F::NP, F::TB, F::THREADS>(s.B, B, p.B_l, t0, tend, p.N, p.seq);
-    stage_rows<T, F::NP, F::TB, F::THREADS>(s.C, C, p.C_l, t0, tend, p.N, p.seq);
+    stage_rows<T, F::NP, F::TB, F::THREADS>(s.B, B, p.B_l, t0, tend, p.N, p.seq, p.quads);
+    stage_rows<T, F::NP, F::TB, F::THREADS>(s.C, C, p.C_l, t0, tend, p.N, p.seq, p.quads);
     __syncthreads();
 
     float h0[NPT], hm[NPT];  // the states before the tile's first token and before its second half
@@ -332,6 +332,7 @@ extern "C" int ttt_selective_scan_bwd(int rows, int L, int D, int G, int N, cons
   p.du = du, p.ddelta = ddelta, p.dz = dz, p.dinit = dinit;
   const int every = scan::save_every(N);
   p.nsave = (L + every - 1) / every;
+  p.quads = scan::quads(p, dt);
   const int nchunks = bwd_pieces(rows, L, D, N);
   const scan::BwdScratch s = scan::bwd_scratch(rows, L, D, G, N, nchunks);
   if ((rc = scan::plan(p, scratch, scratch_bytes, 2 * s.part_bc + s.part_p, who))) return rc;
