@@ -5,7 +5,7 @@ argument's rounding, and the errors of up to L steps add, so L * 2^-21 for value
 recurrence; sums over D channels, N states or M = B * L tokens add (D + N) * 2^-23 resp.
 M * 2^-24 of their terms' size, which random signs make up to sqrt of the count larger than the
 sum: 8 * 2^-24 * (L + D + N) covers both at these sizes. 16-bit outputs are rounded once, half a
-step of their type, on top. dB and dC of 16-bit inputs are sums of products whose two factors
+step of their type, on top. dB and dC of bf16 inputs are sums of products whose two factors
 are rounded to tensor-core operands of 11 bits: 2^-10 of a product's size more.
 """
 
@@ -28,7 +28,7 @@ def tol(dtype, L, D, N, product=False):
     base = tol32(L, D, N)
     if dtype == torch.float32:
         return base
-    return torch.finfo(dtype).eps / 2 + base + (2.0**-10 if product else 0)
+    return torch.finfo(dtype).eps / 2 + base + (2.0**-10 if product and dtype == torch.bfloat16 else 0)
 
 
 def make(B, L, D, N, G, dtype, seed, nseq=None, z=True, skip=True, bias=True):

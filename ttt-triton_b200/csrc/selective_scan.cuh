@@ -30,7 +30,7 @@ struct Params {
   const float* init;   // [sequences, D, N] or NULL
   float* fin;          // [sequences, D, N] or NULL
   void* out;           // [rows, L, D]
-  float* hsave;        // [rows, nsave, D, N]: the state before every TB-th token, or NULL
+  float* hsave;        // [rows, nsave, D, N]: the state before every save_every()-th token, or NULL
   float* cstate;       // [rows, nchunks, D, N]: the state entering each piece (nchunks > 1)
   float* csum;         // [rows, nchunks, D]: the sum of dt over a piece
   // backward
@@ -55,8 +55,8 @@ inline Shape shape_of(int N) {
   if (N <= 64) return {8, 8};
   return {8, 16};
 }
-// Tokens between two saved states: the backward kernel's time tile.
-inline int save_every(int N) { return 64 / shape_of(N).NPT; }
+// Tokens between two saved states: those whose states the backward kernel holds in registers.
+inline int save_every(int N) { return 32 / shape_of(N).NPT; }
 
 __device__ __forceinline__ float step_size(const Params& p, float raw) { return p.softplus ? softplus(raw) : raw; }
 

@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(128) scan_fwd_kernel(const __grid_constant__ P
   const T* B = static_cast<const T*>(p.B) + w.row * p.B_b + w.g * p.B_g;
   const T* C = static_cast<const T*>(p.C) + w.row * p.C_b + w.g * p.C_g;
   T* out = static_cast<T*>(p.out) + ((long long)w.row * p.L + first) * p.D + q.pd;
-  const int every = 64 / NPT;
+  const int every = 32 / NPT;
 
   for (int t0 = tbeg; t0 < tend; t0 += F::TT) {
     T uu[F::PAIRS], zz[F::PAIRS], dd[F::PAIRS];

@@ -4,13 +4,18 @@
 //   dC = sum_d h dy,  dB = sum_d g dt u,  s1 = <g, B>,  s2 = <q, A>
 //   du = dt s1 + D dy,  ddt = u s1 + s2,  dA = sum q dt,  dz = dout y silu'(z)
 //
-// A CTA walks its channels' time axis backwards in tiles of TB tokens, each starting at a
-// state that the forward kept. The tile's states are run forward again, SUB tokens at a time
-// held in registers (decays a and a h[t-1]), then g runs back through them. Sums over a
-// channel's states (s1, s2 and y) go through shared memory, those over channels (dB, dC)
-// through shuffles within a warp and shared memory between warps; what the CTAs of a group
-// have of dB and dC, and what the rows and pieces have of dA, dD and dbias, is written as
-// partials and added in a fixed order afterwards, so that results do not depend on timing.
+// A CTA walks its channels' time axis backwards in tiles of TB tokens. The forward kept the
+// state before every SUB-th token; from there the states are run forward again with the decays
+// a and a h[t-1] held in registers, then g runs back through them. Sums over a channel's
+// states (s1, s2 and y) go through shared memory. Sums over channels (dB, dC) are products of
+// the state matrix h (or g) of a token with its vector dy (or dt u), so the tensor cores take
+// them: one mma.sync of 16 (states of two channel groups) x 4 (channels) per pair of states, the
+// vector in the column of its token and zeros in the others. The factors have 11 bits there:
+// for bf16 inputs they are rounded to that (2^-11 each, against 2^-8 of dB's and dC's own type),
+// for fp16 and fp32 split in two such parts, three products a pair, 2^-21.
+// What the CTAs of a group have of dB and dC, and what the rows and pieces have of dA, dD and
+// dbias, is written as partials and added in a fixed order afterwards, so that results do not
+// depend on timing.
 #include "selective_scan.cuh"
 
 namespace ttt {
@@ -21,45 +26,91 @@ struct Bwd {
   static constexpr int THREADS = 256, WARPS = THREADS / 32;
   static constexpr int DT = THREADS / LN;     // channels of a CTA
   static constexpr int NP = LN * NPT;         // states, padded
-  static constexpr int TB = 64 / NPT;         // tokens of a tile: save_every()
-  static constexpr int SUB = TB / 2;          // tokens whose states are in registers
+  static constexpr int SUB = 32 / NPT;        // tokens whose states are in registers: save_every()
+  static constexpr int TB = 2 * SUB;          // tokens of a tile
+  static constexpr int CG = 8 / LN;           // groups of 4 channels in a warp
+  static constexpr int TS = LN < SUB ? LN : SUB;  // tokens side by side in a product's columns
   static constexpr int PAIRS = TB * DT / THREADS > 0 ? TB * DT / THREADS : 1;
   struct Smem {
     float B[TB * NP], C[TB * NP];
-    float dt[TB * DT], dtu[TB * DT], dy[TB * DT];
-    float s1[TB * THREADS], s2[TB * THREADS], s3[TB * THREADS];
-    float dB[WARPS][TB * NP], dC[WARPS][TB * NP];
+    float4 d[TB * DT];                        // step size twice, step size * input twice
+    float2 dy[TB * DT];                       // twice
+    float2 s12[TB * THREADS];
+    float s3[TB * THREADS];
+    float dB[WARPS * CG][TB * NP], dC[WARPS * CG][TB * NP];
     float red[THREADS];
+    unsigned dt_max[WARPS], A_max[WARPS];
     SeqMask m;
   };
 };
 
-template <typename T, int LN, int NPT>
-__global__ void __launch_bounds__(256) scan_bwd_kernel(const __grid_constant__ Params p) {
+__device__ __forceinline__ float tf32(float x) {
+  unsigned r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return __uint_as_float(r);
+}
+__device__ __forceinline__ void mma_16x8x4(float (&c)[4], float a0, float a1, float b) {
+  asm volatile("mma.sync.aligned.m16n8k4.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(__float_as_uint(a0)), "r"(__float_as_uint(a1)), "r"(__float_as_uint(b)));
+}
+// The 11 leading bits of x, for the split form: x = high + high(x - high) to 2^-21.
+__device__ __forceinline__ float high(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
+// c += v b over the warp's channels, v a pair of states; SPLIT: both factors in two parts.
+template <bool SPLIT>
+__device__ __forceinline__ void add_product(float (&c)[4], float2 v, float b, float b_low) {
+  if constexpr (SPLIT) {
+    const float x = high(v.x), y = high(v.y);
+    const float2 low = __fadd2_rn(v, make_float2(-x, -y));
+    mma_16x8x4(c, high(low.x), high(low.y), b);
+    mma_16x8x4(c, x, y, b_low);
+    mma_16x8x4(c, x, y, b);
+  } else {
+    mma_16x8x4(c, tf32(v.x), tf32(v.y), b);
+  }
+}
+
+template <typename T, int LN, int NPT, bool SEQ>
+__global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const __grid_constant__ Params p) {
   using F = Bwd<LN, NPT>;
+  constexpr bool SPLIT = !std::is_same<T, __nv_bfloat16>::value;
+  constexpr int H = NPT / 2;
   extern __shared__ __align__(16) unsigned char raw_smem[];
   auto& s = *reinterpret_cast<typename F::Smem*>(raw_smem);
   const Where w = where<F::DT>(p);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // lane -> channel and states: the low two bits and those above the LN state threads' are
-  // the channel's
-  const int nl = (lane >> 2) % LN, cl = warp * (32 / LN) + (lane & 3) + 4 * ((lane >> 2) / LN);
-  const int n0 = nl * NPT, at = cl * LN + nl;
+  // lane -> channel and states, as the products' first operand wants them: rows lane / 4 are
+  // (channel group, state run), columns lane % 4 the group's channels
+  const int l3 = lane & 3, row8 = lane >> 2, cg = row8 / LN, nl = row8 % LN;
+  const int cl = warp * (32 / LN) + l3 + 4 * cg, n0 = nl * NPT, at = cl * LN + nl;
+  // and as the second operand wants them: column lane / 4 is (token, channel group)
+  const int col_tok = row8 / F::CG, col_ch = warp * (32 / LN) + l3 + 4 * (row8 % F::CG);
   const int d = w.g * p.Dg + w.d0 + cl;
   const bool on = w.d0 + cl < p.Dg;
-  const int pc = tid % F::DT, pd = w.g * p.Dg + w.d0 + pc;  // channel in the element-wise passes
+  const int pc = tid % F::DT, tq = tid / F::DT, pd = w.g * p.Dg + w.d0 + pc;  // element-wise passes
   const bool pon = w.d0 + pc < p.Dg;
   const int tbeg = w.piece * p.chunk, tend = min(p.L, tbeg + p.chunk);
   const long long DN = (long long)p.D * p.N;
+  const int* seq = SEQ ? p.seq : nullptr;
 
-  float A2[NPT], carry[NPT], dA[NPT];
-  load_states<NPT>(p.A, d, n0, p.N, on, A2);
+  float hs[NPT];
+  load_states<NPT>(p.A, d, n0, p.N, on, hs);
+  float amax = 0.f;
 #pragma unroll
-  for (int i = 0; i < NPT; ++i) A2[i] *= kLog2e, dA[i] = 0.f;
+  for (int i = 0; i < NPT; ++i) {
+    hs[i] *= kLog2e;
+    amax = fabsf(hs[i]) <= amax ? amax : fabsf(hs[i]);
+  }
+  const unsigned am = warp_max_abs(amax);
+  if (lane == 0) s.A_max[warp] = am;
+  const Pairs<NPT> A2 = pairs_of<NPT>(hs);
   if (p.nchunks > 1)
-    load_states<NPT>(p.cstate + ((long long)w.row * p.nchunks + w.piece) * DN, d, n0, p.N, on, carry);
+    load_states<NPT>(p.cstate + ((long long)w.row * p.nchunks + w.piece) * DN, d, n0, p.N, on, hs);
   else
-    load_states<NPT>(p.dfin + w.row * DN, d, n0, p.N, on && p.dfin && !p.seq, carry);
+    load_states<NPT>(p.dfin + w.row * DN, d, n0, p.N, on && p.dfin && !SEQ, hs);
+  Pairs<NPT> carry = pairs_of<NPT>(hs), dA;
+#pragma unroll
+  for (int j = 0; j < H; ++j) dA.v[j] = make_float2(0.f, 0.f);
   const float skip = pon && p.Dskip ? p.Dskip[pd] : 0.f, bias = pon && p.bias ? p.bias[pd] : 0.f;
   const T* u = static_cast<const T*>(p.u) + w.row * p.u_b + pd;
   const T* delta = static_cast<const T*>(p.delta) + w.row * p.delta_b + pd;
@@ -71,116 +122,171 @@ __global__ void __launch_bounds__(256) scan_bwd_kernel(const __grid_constant__ P
 
   for (int tile = (tend - 1) / F::TB; tile >= tbeg / F::TB; --tile) {
     const int t0 = tile * F::TB;
-    float uu[F::PAIRS], raw[F::PAIRS], zz[F::PAIRS], dd[F::PAIRS];
-    if (p.seq) stage_masks<F::TB>(&s.m, p.seq, t0, tend, p.L);
+    T uu[F::PAIRS], rr[F::PAIRS], zz[F::PAIRS], dd[F::PAIRS];
+    if (SEQ) stage_masks<F::TB>(&s.m, p.seq, t0, tend, p.L);
 #pragma unroll
     for (int k = 0; k < F::PAIRS; ++k) {
-      const int t = tid / F::DT + k * LN, tok = t0 + t;
-      float dt = 0.f, dy = 0.f;
-      uu[k] = raw[k] = zz[k] = dd[k] = 0.f;
+      const int t = tq + k * LN, tok = t0 + t;
+      uu[k] = from_f<T>(0.f), rr[k] = zz[k] = dd[k] = uu[k];
+      if (t < F::TB && pon && tok < tend && in_sequence(seq, tok)) {
+        uu[k] = u[tok * p.u_l], rr[k] = delta[tok * p.delta_l];
+        dd[k] = static_cast<const T*>(p.dout)[(row0 + tok) * p.D + pd];
+        if (z) zz[k] = z[tok * p.z_l];
+      }
+    }
+    stage_rows<T, F::NP, F::TB, F::THREADS>(s.B, B, p.B_l, t0, tend, p.N, seq, p.quads);
+    stage_rows<T, F::NP, F::TB, F::THREADS>(s.C, C, p.C_l, t0, tend, p.N, seq, p.quads);
+    float m = 0.f;
+#pragma unroll
+    for (int k = 0; k < F::PAIRS; ++k) {
+      const int t = tq + k * LN, tok = t0 + t;
       if (t < F::TB) {
-        if (pon && tok < tend && !(p.seq && p.seq[tok] < 0)) {
-          uu[k] = to_f(u[tok * p.u_l]);
-          raw[k] = to_f(delta[tok * p.delta_l]) + bias;
-          dt = step_size(p, raw[k]);
-          dd[k] = dy = to_f(static_cast<const T*>(p.dout)[(row0 + tok) * p.D + pd]);
-          if (z) {
-            zz[k] = to_f(z[tok * p.z_l]);
-            dy *= zz[k] * sigmoid(zz[k]);
-          }
+        const bool in = pon && tok < tend && in_sequence(seq, tok);
+        const float dt = in ? step_size(p, to_f(rr[k]) + bias) : 0.f, x = dt * to_f(uu[k]);
+        float dy = to_f(dd[k]);
+        if (z) {
+          const float g = to_f(zz[k]);
+          dy *= g * sigmoid(g);
         }
-        s.dt[t * F::DT + pc] = dt, s.dtu[t * F::DT + pc] = dt * uu[k], s.dy[t * F::DT + pc] = dy;
+        m = fabsf(dt) <= m ? m : fabsf(dt);
+        s.d[t * F::DT + pc] = make_float4(dt, dt, x, x), s.dy[t * F::DT + pc] = make_float2(dy, dy);
       }
     }
-    stage_rows<T, F::NP, F::TB, F::THREADS>(s.B, B, p.B_l, t0, tend, p.N, p.seq, p.quads);
-    stage_rows<T, F::NP, F::TB, F::THREADS>(s.C, C, p.C_l, t0, tend, p.N, p.seq, p.quads);
+    const unsigned wm = warp_max_abs(m);
+    if (lane == 0) s.dt_max[warp] = wm;
     __syncthreads();
+    const bool poly = max_of(s.dt_max) * max_of(s.A_max) < kPolyRange;
 
-    float h0[NPT], hm[NPT];  // the states before the tile's first token and before its second half
-    load_states<NPT>(p.hsave + ((long long)w.row * p.nsave + tile) * DN, d, n0, p.N, on, h0);
-    const auto restart = [&](int t, float (&h)[NPT]) {
-      if (p.seq && (s.m.start >> t & 1)) {
-        const int q = p.seq[t0 + t];
-        load_states<NPT>(p.init + q * DN, d, n0, p.N, on && q >= 0 && p.init, h);
-      }
-    };
-#pragma unroll
-    for (int i = 0; i < NPT; ++i) hm[i] = h0[i];
-#pragma unroll
-    for (int t = 0; t < F::SUB; ++t) {
-      restart(t, hm);
-      const float dt = s.dt[t * F::DT + cl], dtu = s.dtu[t * F::DT + cl];
-#pragma unroll
-      for (int i = 0; i < NPT; ++i)
-        hm[i] = fmaf(ex2(dt * A2[i]), hm[i], dtu * s.B[t * F::NP + n0 + i]);
-    }
 #pragma unroll 1
     for (int half = 1; half >= 0; --half) {
       const int b = half * F::SUB;
-      float a[F::SUB][NPT], ah[F::SUB][NPT], h[NPT];
+      if (t0 + b >= tend) continue;
+      const auto tokens = [&](auto use_poly, auto checks) {
+        float2 a[F::SUB][H], ah[F::SUB][H];
+        Pairs<NPT> h;
+        load_states<NPT>(p.hsave + ((long long)w.row * p.nsave + 2 * tile + half) * DN, d, n0, p.N, on, hs);
+        h = pairs_of<NPT>(hs);
 #pragma unroll
-      for (int i = 0; i < NPT; ++i) h[i] = half ? hm[i] : h0[i];
+        for (int k = 0; k < F::SUB; ++k) {
+          const int t = b + k;
+          if constexpr (decltype(checks)::value) {
+            if (SEQ && (s.m.start >> t & 1)) {
+              const int sq = p.seq[t0 + t];
+              load_states<NPT>(p.init + sq * DN, d, n0, p.N, on && sq >= 0 && p.init, hs);
+              h = pairs_of<NPT>(hs);
+            }
+          }
+          const float4 dd4 = s.d[t * F::DT + cl];
+          const float2 dt = make_float2(dd4.x, dd4.y), dtu = make_float2(dd4.z, dd4.w);
+          const Pairs<NPT> B2 = row_pairs<NPT>(s.B + t * F::NP + n0);
 #pragma unroll
-      for (int k = 0; k < F::SUB; ++k) {
-        const int t = b + k;
-        restart(t, h);
-        const float dt = s.dt[t * F::DT + cl], dtu = s.dtu[t * F::DT + cl];
-#pragma unroll
-        for (int i = 0; i < NPT; ++i) {
-          a[k][i] = ex2(dt * A2[i]);
-          ah[k][i] = a[k][i] * h[i];
-          h[i] = fmaf(dtu, s.B[t * F::NP + n0 + i], ah[k][i]);
+          for (int j = 0; j < H; ++j) {
+            const int i = (k * H + j) % 8;
+            a[k][j] = decltype(use_poly)::value && (i == 1 || i == 5) ? pow2_poly(dt, A2.v[j]) : pow2_unit(dt, A2.v[j]);
+            ah[k][j] = __fmul2_rn(a[k][j], h.v[j]);
+            h.v[j] = __ffma2_rn(dtu, B2.v[j], ah[k][j]);
+          }
         }
-      }
+        // tokens of two sequences never share a product: a NaN of one would reach the other's columns
+        constexpr int TS = decltype(checks)::value ? 1 : F::TS;
+        Pairs<NPT> dA_here;
 #pragma unroll
-      for (int k = F::SUB - 1; k >= 0; --k) {
-        const int t = b + k;
-        const float dt = s.dt[t * F::DT + cl], dtu = s.dtu[t * F::DT + cl], dy = s.dy[t * F::DT + cl];
-        if (p.seq && (s.m.end >> t & 1)) {
-          const int q = p.seq[t0 + t];
-          load_states<NPT>(p.dfin + q * DN, d, n0, p.N, on && q >= 0 && p.dfin, carry);
-        }
-        float s1 = 0.f, s2 = 0.f, s3 = 0.f;
+        for (int j = 0; j < H; ++j) dA_here.v[j] = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < NPT; ++i) {
-          const float Bn = s.B[t * F::NP + n0 + i], Cn = s.C[t * F::NP + n0 + i];
-          const float g = fmaf(Cn, dy, carry[i]), hn = fmaf(dtu, Bn, ah[k][i]), q = g * ah[k][i];
-          s1 = fmaf(g, Bn, s1), s2 = fmaf(q, A2[i], s2), s3 = fmaf(hn, Cn, s3);
-          dA[i] = fmaf(q, dt, dA[i]);
-          carry[i] = a[k][i] * g;
-          float vb = g * dtu, vc = hn * dy;  // summed over the warp's channels
+        for (int g0 = F::SUB - TS; g0 >= 0; g0 -= TS) {
+          float accB[H][4], accC[H][4];
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1)
-            if (o < 4 || o >= 4 * LN)
-              vb += __shfl_xor_sync(0xffffffffu, vb, o), vc += __shfl_xor_sync(0xffffffffu, vc, o);
-          if ((lane & 3) == 0 && (lane >> 2) < LN)
-            s.dB[warp][t * F::NP + n0 + i] = vb, s.dC[warp][t * F::NP + n0 + i] = vc;
+          for (int j = 0; j < H; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) accB[j][e] = accC[j][e] = 0.f;
+          float vB = 0.f, vC = 0.f;  // the products' vectors, in this lane's token and channel
+          if (col_tok < TS) {
+            vB = s.d[(b + g0 + col_tok) * F::DT + col_ch].z;
+            vC = s.dy[(b + g0 + col_tok) * F::DT + col_ch].x;
+          }
+          const float hB = SPLIT ? high(vB) : tf32(vB), hC = SPLIT ? high(vC) : tf32(vC);
+          const float lB = SPLIT ? high(vB - hB) : 0.f, lC = SPLIT ? high(vC - hC) : 0.f;
+#pragma unroll
+          for (int k = g0 + TS - 1; k >= g0; --k) {
+            const int t = b + k;
+            if constexpr (decltype(checks)::value) {
+              if (t0 + t >= tend) continue;
+              if (SEQ && (s.m.end >> t & 1)) {
+                const int sq = p.seq[t0 + t];
+                load_states<NPT>(p.dfin + sq * DN, d, n0, p.N, on && sq >= 0 && p.dfin, hs);
+                carry = pairs_of<NPT>(hs);
+              }
+            }
+            const float4 dd4 = s.d[t * F::DT + cl];
+            const float2 dt = make_float2(dd4.x, dd4.y), dtu = make_float2(dd4.z, dd4.w), dy = s.dy[t * F::DT + cl];
+            const Pairs<NPT> B2 = row_pairs<NPT>(s.B + t * F::NP + n0), C2 = row_pairs<NPT>(s.C + t * F::NP + n0);
+            const bool mine = col_tok == k - g0;
+            const float bB = mine ? hB : 0.f, bC = mine ? hC : 0.f;
+            const float cB = SPLIT && mine ? lB : 0.f, cC = SPLIT && mine ? lC : 0.f;
+            float2 s1 = make_float2(0.f, 0.f), s2 = s1, s3 = s1;
+#pragma unroll
+            for (int j = 0; j < H; ++j) {
+              const float2 g = __ffma2_rn(C2.v[j], dy, carry.v[j]), hn = __ffma2_rn(dtu, B2.v[j], ah[k][j]);
+              const float2 q = __fmul2_rn(g, ah[k][j]);
+              s1 = __ffma2_rn(g, B2.v[j], s1), s2 = __ffma2_rn(q, A2.v[j], s2), s3 = __ffma2_rn(hn, C2.v[j], s3);
+              dA_here.v[j] = __ffma2_rn(q, dt, dA_here.v[j]);
+              carry.v[j] = __fmul2_rn(a[k][j], g);
+              add_product<SPLIT>(accB[j], g, bB, cB);
+              add_product<SPLIT>(accC[j], hn, bC, cC);
+            }
+            s.s12[t * F::THREADS + at] = make_float2(s1.x + s1.y, s2.x + s2.y);
+            s.s3[t * F::THREADS + at] = s3.x + s3.y;
+            if constexpr (decltype(checks)::value) {
+              if (SEQ && p.dinit && (s.m.start >> t & 1)) {
+                const int sq = p.seq[t0 + t];
+                unpair(carry, hs);
+                store_states<NPT>(p.dinit + sq * DN, d, n0, p.N, on && sq >= 0, hs);
+              }
+            }
+          }
+          // of the products' two columns in this lane, those of the row's own channel group
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int c = 2 * l3 + e, tc = c / F::CG;
+            if (c % F::CG == cg && tc < TS) {
+              const int o = (b + g0 + tc) * F::NP + n0;
+#pragma unroll
+              for (int j = 0; j < H; ++j) {
+                *reinterpret_cast<float2*>(&s.dB[warp * F::CG + cg][o + 2 * j]) = make_float2(accB[j][e], accB[j][2 + e]);
+                *reinterpret_cast<float2*>(&s.dC[warp * F::CG + cg][o + 2 * j]) = make_float2(accC[j][e], accC[j][2 + e]);
+              }
+            }
+          }
         }
-        s.s1[t * F::THREADS + at] = s1, s.s2[t * F::THREADS + at] = s2, s.s3[t * F::THREADS + at] = s3;
-        if (p.seq && (s.m.start >> t & 1)) {
-          const int q = p.seq[t0 + t];
-          if (p.dinit) store_states<NPT>(p.dinit + q * DN, d, n0, p.N, on && q >= 0, carry);
-        }
-      }
+#pragma unroll
+        for (int j = 0; j < H; ++j) dA.v[j] = __fadd2_rn(dA.v[j], dA_here.v[j]);
+      };
+      if (t0 + b + F::SUB > tend || (SEQ && ((s.m.start | s.m.end) >> b & ((1u << F::SUB) - 1))))
+        tokens(std::false_type{}, std::true_type{});
+      else if (poly) tokens(std::true_type{}, std::false_type{});
+      else tokens(std::false_type{}, std::false_type{});
     }
     __syncthreads();
 
 #pragma unroll
     for (int k = 0; k < F::PAIRS; ++k) {
-      const int t = tid / F::DT + k * LN, tok = t0 + t;
+      const int t = tq + k * LN, tok = t0 + t;
       if (t < F::TB && pon && tok < tend) {
         float s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
         for (int j = 0; j < LN; ++j) {
           const int e = t * F::THREADS + pc * LN + j;
-          s1 += s.s1[e], s2 += s.s2[e], s3 += s.s3[e];
+          s1 += s.s12[e].x, s2 += s.s12[e].y, s3 += s.s3[e];
         }
-        const float dt = s.dt[t * F::DT + pc], dy = s.dy[t * F::DT + pc];
-        float du = fmaf(dt, s1, skip * dy), ddt = fmaf(uu[k], s1, s2 * kLn2), dz = 0.f;
-        if (p.softplus) ddt *= sigmoid(raw[k]);
-        if (z) dz = dd[k] * fmaf(skip, uu[k], s3) * silu_grad(zz[k], sigmoid(zz[k]));
-        if (p.seq && !(s.m.in >> t & 1)) du = ddt = dz = 0.f;  // a token of no sequence
-        else sum_D = fmaf(uu[k], dy, sum_D), sum_bias += ddt;
+        const float dt = s.d[t * F::DT + pc].x, dy = s.dy[t * F::DT + pc].x, uv = to_f(uu[k]);
+        float du = fmaf(dt, s1, skip * dy), ddt = fmaf(uv, s1, s2 * kLn2), dz = 0.f;
+        if (p.softplus) ddt *= sigmoid(to_f(rr[k]) + bias);
+        if (z) {
+          const float g = to_f(zz[k]);
+          dz = to_f(dd[k]) * fmaf(skip, uv, s3) * silu_grad(g, sigmoid(g));
+        }
+        if (SEQ && !(s.m.in >> t & 1)) du = ddt = dz = 0.f;  // a token of no sequence
+        else sum_D = fmaf(uv, dy, sum_D), sum_bias += ddt;
         const long long o = (row0 + tok) * p.D + pd;
         static_cast<T*>(p.du)[o] = from_f<T>(du);
         static_cast<T*>(p.ddelta)[o] = from_f<T>(ddt);
@@ -193,8 +299,8 @@ __global__ void __launch_bounds__(256) scan_bwd_kernel(const __grid_constant__ P
       if (t0 + t < tend && n < p.N) {
         float vb = 0.f, vc = 0.f;
 #pragma unroll
-        for (int k = 0; k < F::WARPS; ++k) vb += s.dB[k][i], vc += s.dC[k][i];
-        const bool out = p.seq && !(s.m.in >> t & 1);
+        for (int k = 0; k < F::WARPS * F::CG; ++k) vb += s.dB[k][i], vc += s.dC[k][i];
+        const bool out = SEQ && !(s.m.in >> t & 1);
         const long long o = (((long long)tile_g * p.rows * p.L + row0 + t0 + t) * p.G + w.g) * p.N + n;
         p.part_B[o] = out ? 0.f : vb, p.part_C[o] = out ? 0.f : vc;
       }
@@ -202,9 +308,11 @@ __global__ void __launch_bounds__(256) scan_bwd_kernel(const __grid_constant__ P
     __syncthreads();
   }
 
-  if (p.dinit && !p.seq && tbeg == 0) store_states<NPT>(p.dinit + w.row * DN, d, n0, p.N, on, carry);
+  unpair(carry, hs);
+  if (p.dinit && !SEQ && tbeg == 0) store_states<NPT>(p.dinit + w.row * DN, d, n0, p.N, on, hs);
   float* part = p.part_p + ((long long)w.row * p.nchunks + w.piece) * p.D * (p.N + 2);
-  store_states<NPT>(part, d, n0, p.N, on, dA);
+  unpair(dA, hs);
+  store_states<NPT>(part, d, n0, p.N, on, hs);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     s.red[tid] = k ? sum_bias : sum_D;
@@ -272,7 +380,8 @@ template <typename T>
 static int launch_bwd(Params p, void* dB, void* dC, float* dparams, cudaStream_t st, const char* who) {
   int rc = dispatch(p.N, [&](auto ln, auto npt) {
     using F = Bwd<decltype(ln)::value, decltype(npt)::value>;
-    auto kernel = scan_bwd_kernel<T, decltype(ln)::value, decltype(npt)::value>;
+    constexpr int LN = decltype(ln)::value, NPT = decltype(npt)::value;
+    auto kernel = p.seq ? scan_bwd_kernel<T, LN, NPT, true> : scan_bwd_kernel<T, LN, NPT, false>;
     const int rc2 = prepare_smem(kernel, sizeof(typename F::Smem), who);
     if (rc2) return rc2;
     const long long grid = (long long)p.tiles * p.G * p.nchunks * p.rows;
