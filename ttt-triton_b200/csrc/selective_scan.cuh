@@ -26,6 +26,7 @@ struct Params {
   const float *A, *Dskip, *bias;
   int softplus;
   int quads;           // rows of B and C are read four states at a time
+  int couples;         // activations are read and written two channels at a time
   const int* seq;      // packed rows: each token's sequence (rows == 1), else NULL
   const float* init;   // [sequences, D, N] or NULL
   float* fin;          // [sequences, D, N] or NULL
@@ -58,7 +59,6 @@ inline Shape shape_of(int N) {
 // Tokens between two saved states: those whose states the backward kernel holds in registers.
 inline int save_every(int N) { return 32 / shape_of(N).NPT; }
 
-__device__ __forceinline__ float step_size(const Params& p, float raw) { return p.softplus ? softplus(raw) : raw; }
 
 // This thread's NPT states of channel d of a [.., D, N] array (0 past N); in fours where N is a
 // multiple of four and the array lies on a 16-byte boundary, as torch's allocations do.
@@ -121,6 +121,103 @@ __device__ __forceinline__ void stage_rows(float* dst, const T* src, long long l
   }
 }
 
+// Two adjacent channels of an activation. `both`: one access for the two, where every row has
+// them on a boundary of two; else each by itself, where it is there.
+template <typename T>
+struct Two {  // 16-bit types: one register
+  unsigned v;
+};
+template <>
+struct Two<float> {
+  float2 v;
+};
+template <typename T>
+__device__ __forceinline__ Two<T> load_two(const T* p, bool on0, bool on1, bool both) {
+  Two<T> r;
+  if constexpr (std::is_same<T, float>::value) {
+    r.v = make_float2(0.f, 0.f);
+    if (both) {
+      if (on0) r.v = *reinterpret_cast<const float2*>(p);
+    } else {
+      if (on0) r.v.x = p[0];
+      if (on1) r.v.y = p[1];
+    }
+  } else {
+    r.v = 0;
+    if (both) {
+      if (on0) r.v = *reinterpret_cast<const unsigned*>(p);
+    } else {
+      const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+      if (on0) r.v = q[0];
+      if (on1) r.v |= (unsigned)q[1] << 16;
+    }
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ float2 two_f(const Two<T>& r) {
+  if constexpr (std::is_same<T, float>::value) {
+    return r.v;
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    return make_float2(__uint_as_float(r.v << 16), __uint_as_float(r.v & 0xffff0000u));
+  } else {
+    __half2 h;
+    memcpy(&h, &r.v, 4);
+    return __half22float2(h);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_two(T* p, float2 v, bool on0, bool on1, bool both) {
+  if constexpr (std::is_same<T, float>::value) {
+    if (both) {
+      if (on0) *reinterpret_cast<float2*>(p) = v;
+    } else {
+      if (on0) p[0] = v.x;
+      if (on1) p[1] = v.y;
+    }
+  } else {
+    unsigned r;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const __nv_bfloat162 h = __float22bfloat162_rn(v);
+      memcpy(&r, &h, 4);
+    } else {
+      const __half2 h = __float22half2_rn(v);
+      memcpy(&r, &h, 4);
+    }
+    if (both) {
+      if (on0) *reinterpret_cast<unsigned*>(p) = r;
+    } else {
+      unsigned short* q = reinterpret_cast<unsigned short*>(p);
+      if (on0) q[0] = (unsigned short)r;
+      if (on1) q[1] = (unsigned short)(r >> 16);
+    }
+  }
+}
+__device__ __forceinline__ float2 neg2(float2 x) { return make_float2(-x.x, -x.y); }
+__device__ __forceinline__ float2 all2(float x) { return make_float2(x, x); }
+// sigmoid and softplus (scan_common.cuh) of two
+__device__ __forceinline__ float2 sigmoid2(float2 x) {
+  const float2 m = __fmul2_rn(x, all2(-kLog2e));
+  const float2 e = __fadd2_rn(make_float2(ex2(m.x), ex2(m.y)), all2(1.f));
+  return make_float2(rcp(e.x), rcp(e.y));
+}
+__device__ __forceinline__ float2 softplus2(float2 x) {
+  const float2 m = __fmul2_rn(make_float2(fabsf(x.x), fabsf(x.y)), all2(-kLog2e));
+  const float2 w = make_float2(ex2(m.x), ex2(m.y)), e = __fadd2_rn(w, all2(2.f));
+  const float2 s = __fmul2_rn(w, make_float2(rcp(e.x), rcp(e.y))), v = __fmul2_rn(s, s);
+  float2 q = __ffma2_rn(v, all2(0.2814132571220398f), all2(0.2797023057937622f));
+  q = __ffma2_rn(v, q, all2(0.4002406597137451f));
+  q = __ffma2_rn(v, q, all2(0.666663408279419f));
+  q = __ffma2_rn(v, q, all2(2.f));
+  return __ffma2_rn(s, q, make_float2(fmaxf(x.x, 0.f), fmaxf(x.y, 0.f)));
+}
+// x sigmoid(x)
+__device__ __forceinline__ float2 silu2(float2 x) { return __fmul2_rn(x, sigmoid2(x)); }
+// max |x| that keeps a NaN (as integer bits it is above all numbers)
+__device__ __forceinline__ unsigned max_bits(unsigned m, float2 x) {
+  return max(m, max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu));
+}
+
 // NPT states as pairs, and a tile row's values for them.
 template <int NPT>
 struct Pairs {
@@ -145,6 +242,27 @@ __device__ __forceinline__ Pairs<NPT> row_pairs(const float* row) {  // 16-byte 
   for (int j = 0; j < NPT / 4; ++j) {
     const float4 q = reinterpret_cast<const float4*>(row)[j];
     r.v[2 * j] = make_float2(q.x, q.y), r.v[2 * j + 1] = make_float2(q.z, q.w);
+  }
+  return r;
+}
+
+__device__ __forceinline__ float2 params_of(const float* v, int d, bool on0, bool on1) {
+  return make_float2(v && on0 ? v[d] : 0.f, v && on1 ? v[d + 1] : 0.f);
+}
+
+// The sums over the LN threads of two adjacent channels.
+template <int LN>
+__device__ __forceinline__ float2 state_sums(const float* y) {
+  if constexpr (LN == 1) return *reinterpret_cast<const float2*>(y);
+  if constexpr (LN == 2) {
+    const float4 v = *reinterpret_cast<const float4*>(y);
+    return make_float2(v.x + v.y, v.z + v.w);
+  }
+  float2 r = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int j = 0; j < LN / 4; ++j) {
+    const float4 v = reinterpret_cast<const float4*>(y)[j], x = reinterpret_cast<const float4*>(y + LN)[j];
+    r = __fadd2_rn(r, make_float2((v.x + v.y) + (v.z + v.w), (x.x + x.y) + (x.z + x.w)));
   }
   return r;
 }
@@ -174,10 +292,7 @@ __device__ __forceinline__ float2 pow2_unit(float2 dt, float2 A2) {
   return make_float2(ex2(x.x), ex2(x.y));
 }
 
-// The largest |x| of a CTA as integer bits (NaN above all): per warp, for a tile's readers.
-__device__ __forceinline__ unsigned warp_max_abs(float x) {
-  return __reduce_max_sync(0xffffffffu, __float_as_uint(x) & 0x7fffffffu);
-}
+// The largest |x| of a CTA as integer bits: per warp, for a tile's readers.
 template <int WARPS>
 __device__ __forceinline__ float max_of(const unsigned (&m)[WARPS]) {
   unsigned v = m[0];
@@ -209,6 +324,7 @@ int chunk_states(const Params& p, int dt, bool rev, cudaStream_t st, const char*
 // Splits the time axis and lays its part of the scratch out behind `extra` bytes of the caller.
 int plan(Params& p, void* scratch, size_t scratch_bytes, size_t extra, const char* who);
 bool quads(const Params& p, int dt);
+bool couples(const Params& p, int dt);
 size_t plan_bytes(int rows, int L, int D, int N);
 int check_sizes(const char* who, int rows, int L, int D, int G, int N, int dt);
 

@@ -23,7 +23,8 @@ struct Fwd {
   static constexpr int NP = LN * NPT;                // states, padded
   static constexpr int TT = LN >= 4 ? 32 : 8 * LN;   // tokens of a tile
   static constexpr int RUN = 8;                      // tokens unrolled
-  static constexpr int PAIRS = TT * DT / THREADS;    // (token, channel) pairs of a thread
+  static constexpr int TWOS = TT * DT / 2 / THREADS; // couples of channels of a thread, one token each
+  static constexpr int STEP = 2 * LN;                // tokens between them
   struct Smem {
     float B[TT * NP], C[TT * NP];
     float4 d[TT * DT];      // step size twice, step size * input twice: operands of paired arithmetic
@@ -33,22 +34,21 @@ struct Fwd {
   };
 };
 
-// What a thread holds: channel d and states n0 .. in the recurrence; channel pd, and tokens
-// tq, tq + LN, .. of a tile, in the element-wise passes.
+// What a thread holds: channel d and states n0 .. in the recurrence; channels pd, pd + 1, and
+// tokens tq, tq + STEP, .. of a tile, in the element-wise passes.
 template <int LN, int NPT>
 struct Lane {
   int n0, cl, d, tq, pc, pd;
-  bool on, pon;
+  bool on, on0, on1;
   __device__ __forceinline__ Lane(const Params& p, const Where& w) {
     using F = Fwd<LN, NPT>;
     const int tid = threadIdx.x;
     n0 = tid % LN * NPT, cl = tid / LN;
-    pc = tid % F::DT, tq = tid / F::DT;
+    pc = tid % (F::DT / 2) * 2, tq = tid / (F::DT / 2);
     d = w.g * p.Dg + w.d0 + cl, pd = w.g * p.Dg + w.d0 + pc;
-    on = w.d0 + cl < p.Dg, pon = w.d0 + pc < p.Dg;
+    on = w.d0 + cl < p.Dg, on0 = w.d0 + pc < p.Dg, on1 = w.d0 + pc + 1 < p.Dg;
   }
 };
-
 // One token of the recurrence for NPT states; POLY: this token's share of the decays goes to
 // the multiply-add pipes (3 pairs in 8, see pow2_poly).
 template <int NPT, bool POLY>
@@ -78,13 +78,13 @@ __global__ void __launch_bounds__(128) scan_fwd_kernel(const __grid_constant__ P
 
   float hs[NPT];
   load_states<NPT>(p.A, q.d, q.n0, p.N, q.on, hs);
-  float amax = 0.f;
+  unsigned am = 0;
 #pragma unroll
-  for (int i = 0; i < NPT; ++i) {
-    hs[i] *= kLog2e;
-    amax = fabsf(hs[i]) <= amax ? amax : fabsf(hs[i]);  // a NaN stays
+  for (int i = 0; i < NPT; i += 2) {
+    hs[i] *= kLog2e, hs[i + 1] *= kLog2e;
+    am = max_bits(am, make_float2(hs[i], hs[i + 1]));
   }
-  const unsigned am = warp_max_abs(amax);
+  am = __reduce_max_sync(0xffffffffu, am);
   if (tid % 32 == 0) s.A_max[tid / 32] = am;
   const Pairs<NPT> A2 = pairs_of<NPT>(hs);
   if (p.nchunks > 1)
@@ -92,42 +92,45 @@ __global__ void __launch_bounds__(128) scan_fwd_kernel(const __grid_constant__ P
   else
     load_states<NPT>(p.init + w.row * DN, q.d, q.n0, p.N, q.on && p.init && !SEQ, hs);
   Pairs<NPT> h = pairs_of<NPT>(hs);
-  const float skip = q.pon && p.Dskip ? p.Dskip[q.pd] : 0.f, bias = q.pon && p.bias ? p.bias[q.pd] : 0.f;
+  const float2 skip = params_of(p.Dskip, q.pd, q.on0, q.on1), bias = params_of(p.bias, q.pd, q.on0, q.on1);
   const long long first = tbeg + q.tq;
   const T* u = static_cast<const T*>(p.u) + w.row * p.u_b + first * p.u_l + q.pd;
   const T* delta = static_cast<const T*>(p.delta) + w.row * p.delta_b + first * p.delta_l + q.pd;
-  const T* z = p.z ? static_cast<const T*>(p.z) + w.row * p.z_b + first * p.z_l + q.pd : nullptr;
+  const T* z = static_cast<const T*>(p.z) + w.row * p.z_b + first * p.z_l + q.pd;
   const T* B = static_cast<const T*>(p.B) + w.row * p.B_b + w.g * p.B_g;
   const T* C = static_cast<const T*>(p.C) + w.row * p.C_b + w.g * p.C_g;
   T* out = static_cast<T*>(p.out) + ((long long)w.row * p.L + first) * p.D + q.pd;
+  const long long u_step = F::STEP * p.u_l, delta_step = F::STEP * p.delta_l, z_step = F::STEP * p.z_l;
+  const long long out_step = (long long)F::STEP * p.D;
   const int every = 32 / NPT;
 
   for (int t0 = tbeg; t0 < tend; t0 += F::TT) {
-    T uu[F::PAIRS], zz[F::PAIRS], dd[F::PAIRS];
+    Two<T> uu[F::TWOS], zz[F::TWOS], dd[F::TWOS];
     if (SEQ) stage_masks<F::TT>(&s.m, p.seq, t0, tend, p.L);
 #pragma unroll
-    for (int k = 0; k < F::PAIRS; ++k) {
-      const int tok = t0 + q.tq + k * LN;
-      const bool on = q.pon && tok < tend && in_sequence(seq, tok);
-      dd[k] = from_f<T>(0.f), uu[k] = zz[k] = dd[k];
-      if (on) {
-        dd[k] = delta[k * LN * p.delta_l], uu[k] = u[k * LN * p.u_l];
-        if (z) zz[k] = z[k * LN * p.z_l];
-      }
+    for (int k = 0; k < F::TWOS; ++k) {
+      const int tok = t0 + q.tq + k * F::STEP;
+      const bool in = tok < tend && in_sequence(seq, tok), on0 = in && q.on0, on1 = in && q.on1;
+      dd[k] = load_two(delta, on0, on1, p.couples), uu[k] = load_two(u, on0, on1, p.couples);
+      zz[k] = load_two(z, on0 && p.z, on1 && p.z, p.couples);
+      delta += delta_step, u += u_step, z += z_step;
     }
     stage_rows<T, F::NP, F::TT, F::THREADS>(s.B, B, p.B_l, t0, tend, p.N, seq, p.quads);
     stage_rows<T, F::NP, F::TT, F::THREADS>(s.C, C, p.C_l, t0, tend, p.N, seq, p.quads);
-    float m = 0.f;
+    unsigned m = 0;
 #pragma unroll
-    for (int k = 0; k < F::PAIRS; ++k) {
-      const int tok = t0 + q.tq + k * LN;
-      const bool on = q.pon && tok < tend && in_sequence(seq, tok);
-      const float dt = on ? step_size(p, to_f(dd[k]) + bias) : 0.f, x = dt * to_f(uu[k]);
-      m = fabsf(dt) <= m ? m : fabsf(dt);
-      s.d[(q.tq + k * LN) * F::DT + q.pc] = make_float4(dt, dt, x, x);
+    for (int k = 0; k < F::TWOS; ++k) {
+      const int t = q.tq + k * F::STEP, tok = t0 + t;
+      float2 dt = __fadd2_rn(two_f(dd[k]), bias);
+      if (p.softplus) dt = softplus2(dt);
+      if (!(tok < tend && in_sequence(seq, tok))) dt = all2(0.f);
+      const float2 x = __fmul2_rn(dt, two_f(uu[k]));
+      m = max_bits(m, dt);
+      s.d[t * F::DT + q.pc] = make_float4(dt.x, dt.x, x.x, x.x);
+      s.d[t * F::DT + q.pc + 1] = make_float4(dt.y, dt.y, x.y, x.y);
     }
-    const unsigned wm = warp_max_abs(m);
-    if (tid % 32 == 0) s.dt_max[tid / 32] = wm;
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (tid % 32 == 0) s.dt_max[tid / 32] = m;
     __syncthreads();
     const bool poly = max_of(s.dt_max) * max_of(s.A_max) < kPolyRange;
 
@@ -178,31 +181,14 @@ __global__ void __launch_bounds__(128) scan_fwd_kernel(const __grid_constant__ P
     __syncthreads();
 
 #pragma unroll
-    for (int k = 0; k < F::PAIRS; ++k) {
-      const int t = q.tq + k * LN, tok = t0 + t;
-      if (q.pon && tok < tend) {
-        float y = 0.f;
-        if constexpr (LN >= 4) {
-#pragma unroll
-          for (int j = 0; j < LN / 4; ++j) {
-            const float4 v = reinterpret_cast<const float4*>(s.y + t * F::THREADS + q.pc * LN)[j];
-            y += (v.x + v.y) + (v.z + v.w);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < LN; ++j) y += s.y[t * F::THREADS + q.pc * LN + j];
-        }
-        y = fmaf(skip, to_f(uu[k]), y);
-        if (z) {
-          const float g = to_f(zz[k]);
-          y *= g * sigmoid(g);
-        }
-        if (SEQ && !(s.m.in >> t & 1)) y = 0.f;  // a token of no sequence
-        out[(long long)k * LN * p.D] = from_f<T>(y);
-      }
+    for (int k = 0; k < F::TWOS; ++k) {
+      const int t = q.tq + k * F::STEP, tok = t0 + t;
+      float2 y = __ffma2_rn(skip, two_f(uu[k]), state_sums<LN>(s.y + t * F::THREADS + q.pc * LN));
+      if (p.z) y = __fmul2_rn(y, silu2(two_f(zz[k])));
+      if (SEQ && !(s.m.in >> t & 1)) y = all2(0.f);  // a token of no sequence
+      store_two(out, y, q.on0 && tok < tend, q.on1 && tok < tend, p.couples);
+      out += out_step;
     }
-    u += F::TT * p.u_l, delta += F::TT * p.delta_l, out += (long long)F::TT * p.D;
-    if (z) z += F::TT * p.z_l;
     if (SEQ) __syncthreads();  // the masks are written again
   }
   if (!SEQ && p.fin && tend == p.L) {
@@ -225,26 +211,27 @@ __global__ void __launch_bounds__(128) scan_chunk_kernel(const __grid_constant__
   const long long DN = (long long)p.D * p.N;
   const int* seq = SEQ ? p.seq : nullptr;
 
-  float hs[NPT], sum = 0.f, amax = 0.f;
+  float hs[NPT], sum = 0.f;
   load_states<NPT>(p.A, q.d, q.n0, p.N, q.on, hs);
+  unsigned am = 0;
 #pragma unroll
-  for (int i = 0; i < NPT; ++i) {
-    hs[i] *= kLog2e;
-    amax = fabsf(hs[i]) <= amax ? amax : fabsf(hs[i]);
+  for (int i = 0; i < NPT; i += 2) {
+    hs[i] *= kLog2e, hs[i + 1] *= kLog2e;
+    am = max_bits(am, make_float2(hs[i], hs[i + 1]));
   }
-  const unsigned am = warp_max_abs(amax);
+  am = __reduce_max_sync(0xffffffffu, am);
   if (tid % 32 == 0) s.A_max[tid / 32] = am;
   const Pairs<NPT> A2 = pairs_of<NPT>(hs);
   Pairs<NPT> h;
 #pragma unroll
   for (int j = 0; j < NPT / 2; ++j) h.v[j] = make_float2(0.f, 0.f);
-  const float bias = q.pon && p.bias ? p.bias[q.pd] : 0.f;
+  const float2 bias = params_of(p.bias, q.pd, q.on0, q.on1);
   const T* delta = static_cast<const T*>(p.delta) + w.row * p.delta_b + q.pd;
   // what drives the recurrence: u and B, or dout (gated) and C
   const T* v = REV ? static_cast<const T*>(p.dout) + (long long)w.row * p.L * p.D + q.pd
                    : static_cast<const T*>(p.u) + w.row * p.u_b + q.pd;
   const long long v_l = REV ? p.D : p.u_l;
-  const T* z = REV && p.z ? static_cast<const T*>(p.z) + w.row * p.z_b + q.pd : nullptr;
+  const T* z = static_cast<const T*>(p.z) + w.row * p.z_b + q.pd;
   const T* R = REV ? static_cast<const T*>(p.C) + w.row * p.C_b + w.g * p.C_g
                    : static_cast<const T*>(p.B) + w.row * p.B_b + w.g * p.B_g;
   const long long r_l = REV ? p.C_l : p.B_l;
@@ -254,35 +241,31 @@ __global__ void __launch_bounds__(128) scan_chunk_kernel(const __grid_constant__
   for (int k0 = 0; k0 < ntiles; ++k0) {
     const int t0 = tbeg + (REV ? ntiles - 1 - k0 : k0) * F::TT;
     if (SEQ) stage_masks<F::TT>(&s.m, p.seq, t0, tend, p.L);
-    T dd[F::PAIRS], vv[F::PAIRS], zz[F::PAIRS];
+    Two<T> dd[F::TWOS], vv[F::TWOS], zz[F::TWOS];
 #pragma unroll
-    for (int k = 0; k < F::PAIRS; ++k) {
-      const int tok = t0 + q.tq + k * LN;
-      const bool on = q.pon && tok < tend && in_sequence(seq, tok);
-      dd[k] = from_f<T>(0.f), vv[k] = zz[k] = dd[k];
-      if (on) {
-        dd[k] = delta[tok * p.delta_l], vv[k] = v[tok * v_l];
-        if (REV && z) zz[k] = z[tok * p.z_l];
-      }
+    for (int k = 0; k < F::TWOS; ++k) {
+      const int tok = t0 + q.tq + k * F::STEP;
+      const bool in = tok < tend && in_sequence(seq, tok), on0 = in && q.on0, on1 = in && q.on1;
+      dd[k] = load_two(delta + tok * p.delta_l, on0, on1, p.couples);
+      vv[k] = load_two(v + tok * v_l, on0, on1, p.couples);
+      if (REV) zz[k] = load_two(z + tok * p.z_l, on0 && p.z, on1 && p.z, p.couples);
     }
     stage_rows<T, F::NP, F::TT, F::THREADS>(s.B, R, r_l, t0, tend, p.N, seq, p.quads);
-    float m = 0.f;
+    unsigned m = 0;
 #pragma unroll
-    for (int k = 0; k < F::PAIRS; ++k) {
-      const int tok = t0 + q.tq + k * LN;
-      const bool on = q.pon && tok < tend && in_sequence(seq, tok);
-      const float dt = on ? step_size(p, to_f(dd[k]) + bias) : 0.f;
-      float x = to_f(vv[k]);
-      if (REV && z) {
-        const float g = to_f(zz[k]);
-        x *= g * sigmoid(g);
-      }
-      if (!REV) x *= dt;
-      m = fabsf(dt) <= m ? m : fabsf(dt);
-      s.d[(q.tq + k * LN) * F::DT + q.pc] = make_float4(dt, dt, x, x);
+    for (int k = 0; k < F::TWOS; ++k) {
+      const int t = q.tq + k * F::STEP, tok = t0 + t;
+      float2 dt = __fadd2_rn(two_f(dd[k]), bias), x = two_f(vv[k]);
+      if (p.softplus) dt = softplus2(dt);
+      if (!(tok < tend && in_sequence(seq, tok))) dt = all2(0.f);
+      if (REV && p.z) x = __fmul2_rn(x, silu2(two_f(zz[k])));
+      if (!REV) x = __fmul2_rn(x, dt);
+      m = max_bits(m, dt);
+      s.d[t * F::DT + q.pc] = make_float4(dt.x, dt.x, x.x, x.x);
+      s.d[t * F::DT + q.pc + 1] = make_float4(dt.y, dt.y, x.y, x.y);
     }
-    const unsigned wm = warp_max_abs(m);
-    if (tid % 32 == 0) s.dt_max[tid / 32] = wm;
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (tid % 32 == 0) s.dt_max[tid / 32] = m;
     __syncthreads();
     const bool poly = max_of(s.dt_max) * max_of(s.A_max) < kPolyRange;
 
@@ -485,6 +468,18 @@ bool quads(const Params& p, int dt) {
   return reinterpret_cast<uintptr_t>(p.B) % (4 * elem) == 0 && reinterpret_cast<uintptr_t>(p.C) % (4 * elem) == 0;
 }
 
+// Whether activations may be read and written two channels at a time.
+bool couples(const Params& p, int dt) {
+  const int two = dt == DT_F32 ? 8 : 4;
+  if (p.Dg % 2) return false;
+  for (const long long st : {p.u_b, p.u_l, p.delta_b, p.delta_l, p.z_b, p.z_l})
+    if (st % 2) return false;
+  for (const void* q : {p.u, p.delta, p.z, (const void*)p.out, p.dout, (const void*)p.du, (const void*)p.ddelta,
+                        (const void*)p.dz})
+    if (reinterpret_cast<uintptr_t>(q) % two) return false;
+  return true;
+}
+
 // Pieces of the time axis: as many as bring the device about two full waves of warps, no
 // piece under 64 tokens.
 int pieces(int rows, int L, int D, int N) {
@@ -568,7 +563,7 @@ extern "C" int ttt_selective_scan_fwd(int rows, int L, int D, int G, int N, cons
   p.seq = seq, p.init = init, p.fin = fin, p.out = out, p.hsave = saved;
   const int every = scan::save_every(N);
   p.nsave = (L + every - 1) / every;
-  p.quads = scan::quads(p, dt);
+  p.quads = scan::quads(p, dt), p.couples = scan::couples(p, dt);
   if ((rc = scan::plan(p, scratch, scratch_bytes, 0, who))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (p.nchunks > 1 && (rc = scan::chunk_states(p, dt, false, st, who))) return rc;

@@ -30,7 +30,8 @@ struct Bwd {
   static constexpr int TB = 2 * SUB;          // tokens of a tile
   static constexpr int CG = 8 / LN;           // groups of 4 channels in a warp
   static constexpr int TS = LN < SUB ? LN : SUB;  // tokens side by side in a product's columns
-  static constexpr int PAIRS = TB * DT / THREADS > 0 ? TB * DT / THREADS : 1;
+  static constexpr int TWOS = TB * DT / 2 / THREADS > 0 ? TB * DT / 2 / THREADS : 1;  // couples of a thread
+  static constexpr int STEP = 2 * LN;         // tokens between them
   struct Smem {
     float B[TB * NP], C[TB * NP];
     float4 d[TB * DT];                        // step size twice, step size * input twice
@@ -38,7 +39,7 @@ struct Bwd {
     float2 s12[TB * THREADS];
     float s3[TB * THREADS];
     float dB[WARPS * CG][TB * NP], dC[WARPS * CG][TB * NP];
-    float red[THREADS];
+    float2 red[THREADS];
     unsigned dt_max[WARPS], A_max[WARPS];
     SeqMask m;
   };
@@ -87,21 +88,22 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
   const int col_tok = row8 / F::CG, col_ch = warp * (32 / LN) + l3 + 4 * (row8 % F::CG);
   const int d = w.g * p.Dg + w.d0 + cl;
   const bool on = w.d0 + cl < p.Dg;
-  const int pc = tid % F::DT, tq = tid / F::DT, pd = w.g * p.Dg + w.d0 + pc;  // element-wise passes
-  const bool pon = w.d0 + pc < p.Dg;
+  // channels pd, pd + 1 and tokens tq, tq + STEP, .. of a tile in the element-wise passes
+  const int pc = tid % (F::DT / 2) * 2, tq = tid / (F::DT / 2), pd = w.g * p.Dg + w.d0 + pc;
+  const bool on0 = w.d0 + pc < p.Dg, on1 = w.d0 + pc + 1 < p.Dg;
   const int tbeg = w.piece * p.chunk, tend = min(p.L, tbeg + p.chunk);
   const long long DN = (long long)p.D * p.N;
   const int* seq = SEQ ? p.seq : nullptr;
 
   float hs[NPT];
   load_states<NPT>(p.A, d, n0, p.N, on, hs);
-  float amax = 0.f;
+  unsigned am = 0;
 #pragma unroll
-  for (int i = 0; i < NPT; ++i) {
-    hs[i] *= kLog2e;
-    amax = fabsf(hs[i]) <= amax ? amax : fabsf(hs[i]);
+  for (int i = 0; i < NPT; i += 2) {
+    hs[i] *= kLog2e, hs[i + 1] *= kLog2e;
+    am = max_bits(am, make_float2(hs[i], hs[i + 1]));
   }
-  const unsigned am = warp_max_abs(amax);
+  am = __reduce_max_sync(0xffffffffu, am);
   if (lane == 0) s.A_max[warp] = am;
   const Pairs<NPT> A2 = pairs_of<NPT>(hs);
   if (p.nchunks > 1)
@@ -111,49 +113,53 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
   Pairs<NPT> carry = pairs_of<NPT>(hs), dA;
 #pragma unroll
   for (int j = 0; j < H; ++j) dA.v[j] = make_float2(0.f, 0.f);
-  const float skip = pon && p.Dskip ? p.Dskip[pd] : 0.f, bias = pon && p.bias ? p.bias[pd] : 0.f;
+  const float2 skip = params_of(p.Dskip, pd, on0, on1), bias = params_of(p.bias, pd, on0, on1);
   const T* u = static_cast<const T*>(p.u) + w.row * p.u_b + pd;
   const T* delta = static_cast<const T*>(p.delta) + w.row * p.delta_b + pd;
-  const T* z = p.z ? static_cast<const T*>(p.z) + w.row * p.z_b + pd : nullptr;
+  const T* z = static_cast<const T*>(p.z) + w.row * p.z_b + pd;
+  const T* dout = static_cast<const T*>(p.dout) + (long long)w.row * p.L * p.D + pd;
   const T* B = static_cast<const T*>(p.B) + w.row * p.B_b + w.g * p.B_g;
   const T* C = static_cast<const T*>(p.C) + w.row * p.C_b + w.g * p.C_g;
   const long long row0 = (long long)w.row * p.L;
-  float sum_D = 0.f, sum_bias = 0.f;
+  const float* kept = p.hsave + (long long)w.row * p.nsave * DN;
+  float2 sum_D = all2(0.f), sum_bias = all2(0.f);
 
   for (int tile = (tend - 1) / F::TB; tile >= tbeg / F::TB; --tile) {
     const int t0 = tile * F::TB;
-    T uu[F::PAIRS], rr[F::PAIRS], zz[F::PAIRS], dd[F::PAIRS];
+    Two<T> uu[F::TWOS], rr[F::TWOS], zz[F::TWOS], dd[F::TWOS];
     if (SEQ) stage_masks<F::TB>(&s.m, p.seq, t0, tend, p.L);
 #pragma unroll
-    for (int k = 0; k < F::PAIRS; ++k) {
-      const int t = tq + k * LN, tok = t0 + t;
-      uu[k] = from_f<T>(0.f), rr[k] = zz[k] = dd[k] = uu[k];
-      if (t < F::TB && pon && tok < tend && in_sequence(seq, tok)) {
-        uu[k] = u[tok * p.u_l], rr[k] = delta[tok * p.delta_l];
-        dd[k] = static_cast<const T*>(p.dout)[(row0 + tok) * p.D + pd];
-        if (z) zz[k] = z[tok * p.z_l];
-      }
+    for (int k = 0; k < F::TWOS; ++k) {
+      const int t = tq + k * F::STEP, tok = t0 + t;
+      const bool in = t < F::TB && tok < tend && in_sequence(seq, tok), i0 = in && on0, i1 = in && on1;
+      uu[k] = load_two(u + tok * p.u_l, i0, i1, p.couples), rr[k] = load_two(delta + tok * p.delta_l, i0, i1, p.couples);
+      dd[k] = load_two(dout + (long long)tok * p.D, i0, i1, p.couples);
+      zz[k] = load_two(z + tok * p.z_l, i0 && p.z, i1 && p.z, p.couples);
     }
+    // the states before the tile's halves
+    float h_kept[2][NPT];
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+      load_states<NPT>(kept + (2 * tile + half) * DN, d, n0, p.N, on && t0 + half * F::SUB < tend, h_kept[half]);
     stage_rows<T, F::NP, F::TB, F::THREADS>(s.B, B, p.B_l, t0, tend, p.N, seq, p.quads);
     stage_rows<T, F::NP, F::TB, F::THREADS>(s.C, C, p.C_l, t0, tend, p.N, seq, p.quads);
-    float m = 0.f;
+    unsigned m = 0;
 #pragma unroll
-    for (int k = 0; k < F::PAIRS; ++k) {
-      const int t = tq + k * LN, tok = t0 + t;
+    for (int k = 0; k < F::TWOS; ++k) {
+      const int t = tq + k * F::STEP, tok = t0 + t;
       if (t < F::TB) {
-        const bool in = pon && tok < tend && in_sequence(seq, tok);
-        const float dt = in ? step_size(p, to_f(rr[k]) + bias) : 0.f, x = dt * to_f(uu[k]);
-        float dy = to_f(dd[k]);
-        if (z) {
-          const float g = to_f(zz[k]);
-          dy *= g * sigmoid(g);
-        }
-        m = fabsf(dt) <= m ? m : fabsf(dt);
-        s.d[t * F::DT + pc] = make_float4(dt, dt, x, x), s.dy[t * F::DT + pc] = make_float2(dy, dy);
+        float2 dt = __fadd2_rn(two_f(rr[k]), bias), dy = two_f(dd[k]);
+        if (p.softplus) dt = softplus2(dt);
+        if (!(tok < tend && in_sequence(seq, tok))) dt = all2(0.f);
+        const float2 x = __fmul2_rn(dt, two_f(uu[k]));
+        if (p.z) dy = __fmul2_rn(dy, silu2(two_f(zz[k])));
+        m = max_bits(m, dt);
+        s.d[t * F::DT + pc] = make_float4(dt.x, dt.x, x.x, x.x), s.d[t * F::DT + pc + 1] = make_float4(dt.y, dt.y, x.y, x.y);
+        *reinterpret_cast<float4*>(&s.dy[t * F::DT + pc]) = make_float4(dy.x, dy.x, dy.y, dy.y);
       }
     }
-    const unsigned wm = warp_max_abs(m);
-    if (lane == 0) s.dt_max[warp] = wm;
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) s.dt_max[warp] = m;
     __syncthreads();
     const bool poly = max_of(s.dt_max) * max_of(s.A_max) < kPolyRange;
 
@@ -164,7 +170,8 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
       const auto tokens = [&](auto use_poly, auto checks) {
         float2 a[F::SUB][H], ah[F::SUB][H];
         Pairs<NPT> h;
-        load_states<NPT>(p.hsave + ((long long)w.row * p.nsave + 2 * tile + half) * DN, d, n0, p.N, on, hs);
+#pragma unroll
+        for (int i = 0; i < NPT; ++i) hs[i] = half ? h_kept[1][i] : h_kept[0][i];
         h = pairs_of<NPT>(hs);
 #pragma unroll
         for (int k = 0; k < F::SUB; ++k) {
@@ -269,28 +276,34 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
     __syncthreads();
 
 #pragma unroll
-    for (int k = 0; k < F::PAIRS; ++k) {
-      const int t = tq + k * LN, tok = t0 + t;
-      if (t < F::TB && pon && tok < tend) {
-        float s1 = 0.f, s2 = 0.f, s3 = 0.f;
+    for (int k = 0; k < F::TWOS; ++k) {
+      const int t = tq + k * F::STEP, tok = t0 + t;
+      if (t < F::TB && tok < tend && on0) {
+        // sums over the states: s1, s2 of the two channels, then y
+        float4 s12 = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int j = 0; j < LN; ++j) {
-          const int e = t * F::THREADS + pc * LN + j;
-          s1 += s.s12[e].x, s2 += s.s12[e].y, s3 += s.s3[e];
+          const float2 x = s.s12[t * F::THREADS + pc * LN + j], y = s.s12[t * F::THREADS + (pc + 1) * LN + j];
+          s12.x += x.x, s12.y += y.x, s12.z += x.y, s12.w += y.y;
         }
-        const float dt = s.d[t * F::DT + pc].x, dy = s.dy[t * F::DT + pc].x, uv = to_f(uu[k]);
-        float du = fmaf(dt, s1, skip * dy), ddt = fmaf(uv, s1, s2 * kLn2), dz = 0.f;
-        if (p.softplus) ddt *= sigmoid(to_f(rr[k]) + bias);
-        if (z) {
-          const float g = to_f(zz[k]);
-          dz = to_f(dd[k]) * fmaf(skip, uv, s3) * silu_grad(g, sigmoid(g));
+        const float2 s1 = make_float2(s12.x, s12.y), s2 = make_float2(s12.z, s12.w);
+        const float2 s3 = state_sums<LN>(s.s3 + t * F::THREADS + pc * LN);
+        const float2 dt = make_float2(s.d[t * F::DT + pc].x, s.d[t * F::DT + pc + 1].x), uv = two_f(uu[k]);
+        const float2 dy = make_float2(s.dy[t * F::DT + pc].x, s.dy[t * F::DT + pc + 1].x);
+        float2 du = __ffma2_rn(dt, s1, __fmul2_rn(skip, dy)), ddt = __ffma2_rn(uv, s1, __fmul2_rn(s2, all2(kLn2)));
+        float2 dz = all2(0.f);
+        if (p.softplus) ddt = __fmul2_rn(ddt, sigmoid2(__fadd2_rn(two_f(rr[k]), bias)));
+        if (p.z) {  // silu'(g) = s (1 + g (1 - s))
+          const float2 g = two_f(zz[k]), sg = sigmoid2(g);
+          const float2 slope = __fmul2_rn(sg, __ffma2_rn(g, __fadd2_rn(all2(1.f), neg2(sg)), all2(1.f)));
+          dz = __fmul2_rn(__fmul2_rn(two_f(dd[k]), slope), __ffma2_rn(skip, uv, s3));
         }
-        if (SEQ && !(s.m.in >> t & 1)) du = ddt = dz = 0.f;  // a token of no sequence
-        else sum_D = fmaf(uv, dy, sum_D), sum_bias += ddt;
+        if (SEQ && !(s.m.in >> t & 1)) du = ddt = dz = all2(0.f);  // a token of no sequence
+        else sum_D = __ffma2_rn(uv, dy, sum_D), sum_bias = __fadd2_rn(sum_bias, ddt);
         const long long o = (row0 + tok) * p.D + pd;
-        static_cast<T*>(p.du)[o] = from_f<T>(du);
-        static_cast<T*>(p.ddelta)[o] = from_f<T>(ddt);
-        if (z) static_cast<T*>(p.dz)[o] = from_f<T>(dz);
+        store_two(static_cast<T*>(p.du) + o, du, true, on1, p.couples);
+        store_two(static_cast<T*>(p.ddelta) + o, ddt, true, on1, p.couples);
+        if (p.z) store_two(static_cast<T*>(p.dz) + o, dz, true, on1, p.couples);
       }
     }
     const int tile_g = w.d0 / F::DT;
@@ -317,11 +330,12 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
   for (int k = 0; k < 2; ++k) {
     s.red[tid] = k ? sum_bias : sum_D;
     __syncthreads();
-    if (tid < F::DT && pon) {
-      float v = 0.f;
+    if (tid < F::DT / 2) {
+      float2 v = all2(0.f);
 #pragma unroll
-      for (int j = 0; j < LN; ++j) v += s.red[tid + j * F::DT];
-      part[DN + (long long)k * p.D + pd] = v;
+      for (int j = 0; j < F::STEP; ++j) v = __fadd2_rn(v, s.red[tid + j * (F::DT / 2)]);
+      if (on0) part[DN + (long long)k * p.D + pd] = v.x;
+      if (on1) part[DN + (long long)k * p.D + pd + 1] = v.y;
     }
     __syncthreads();
   }
@@ -441,7 +455,7 @@ extern "C" int ttt_selective_scan_bwd(int rows, int L, int D, int G, int N, cons
   p.du = du, p.ddelta = ddelta, p.dz = dz, p.dinit = dinit;
   const int every = scan::save_every(N);
   p.nsave = (L + every - 1) / every;
-  p.quads = scan::quads(p, dt);
+  p.quads = scan::quads(p, dt), p.couples = scan::couples(p, dt);
   const int nchunks = bwd_pieces(rows, L, D, N);
   const scan::BwdScratch s = scan::bwd_scratch(rows, L, D, G, N, nchunks);
   if ((rc = scan::plan(p, scratch, scratch_bytes, 2 * s.part_bc + s.part_p, who))) return rc;
