@@ -57,7 +57,8 @@ inline Shape shape_of(int N) {
   return {8, 16};
 }
 // Tokens between two saved states: those whose states the backward kernel holds in registers.
-inline int save_every(int N) { return 32 / shape_of(N).NPT; }
+__host__ __device__ constexpr int save_every_of(int NPT) { return NPT == 4 ? 4 : 32 / NPT; }
+inline int save_every(int N) { return save_every_of(shape_of(N).NPT); }
 
 
 // This thread's NPT states of channel d of a [.., D, N] array (0 past N); in fours where N is a
@@ -91,34 +92,52 @@ __device__ __forceinline__ void store_states(float* base, int d, int n0, int N, 
     if (on && n0 + i < N) p[i] = h[i];
 }
 
-// Stages rows t0 .. t0 + TT - 1 of B or C as fp32 in shared memory (0 past the end, past N and
-// for tokens of no sequence). `quads`: four states at a time, where every row is N = NP states
-// on a boundary of four.
+// Rows t0 .. t0 + TT - 1 of B or C on their way to shared memory as fp32 (0 past the end, past
+// N and for tokens of no sequence): fetch() has four states at a time in registers, where
+// every row is N = NP states on a boundary of four (`quads`); put() writes them, or reads and
+// writes state by state.
+template <typename T, int NP, int TT, int THREADS>
+struct Rows {
+  static constexpr int Q = (TT * NP / 4 + THREADS - 1) / THREADS;
+  struct alignas(4 * sizeof(T)) Quad {
+    T v[4];
+  };
+  Quad q[Q];
+  __device__ __forceinline__ void fetch(int tid, const T* src, long long ld, int t0, int t1, const int* seq, bool quads) {
+#pragma unroll
+    for (int k = 0; k < Q; ++k) {
+      const int i = tid + k * THREADS, t = i / (NP / 4), n = i % (NP / 4) * 4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[k].v[e] = from_f<T>(0.f);
+      if (quads && (TT * NP / 4 % THREADS == 0 || i < TT * NP / 4) && t0 + t < t1 && !(seq && seq[t0 + t] < 0))
+        q[k] = *reinterpret_cast<const Quad*>(src + (t0 + t) * ld + n);
+    }
+  }
+  __device__ __forceinline__ void put(int tid, float* dst, const T* src, long long ld, int t0, int t1, int N, const int* seq,
+                                      bool quads) const {
+    if (quads) {
+#pragma unroll
+      for (int k = 0; k < Q; ++k) {
+        const int i = tid + k * THREADS;
+        if (TT * NP / 4 % THREADS == 0 || i < TT * NP / 4)
+          *reinterpret_cast<float4*>(dst + i * 4) =
+              make_float4(to_f(q[k].v[0]), to_f(q[k].v[1]), to_f(q[k].v[2]), to_f(q[k].v[3]));
+      }
+      return;
+    }
+    for (int i = tid; i < TT * NP; i += THREADS) {
+      const int t = i / NP, n = i - t * NP;
+      dst[i] = t0 + t < t1 && n < N && !(seq && seq[t0 + t] < 0) ? to_f(src[(t0 + t) * ld + n]) : 0.f;
+    }
+  }
+};
+// Both at once.
 template <typename T, int NP, int TT, int THREADS>
 __device__ __forceinline__ void stage_rows(float* dst, const T* src, long long ld, int t0, int t1, int N,
                                            const int* seq, bool quads) {
-  if (quads) {
-    struct alignas(4 * sizeof(T)) Quad {
-      T v[4];
-    };
-#pragma unroll
-    for (int k = 0; k < (TT * NP / 4 + THREADS - 1) / THREADS; ++k) {
-      const int i = threadIdx.x + k * THREADS, t = i / (NP / 4), n = i % (NP / 4) * 4;
-      if (TT * NP / 4 % THREADS == 0 || i < TT * NP / 4) {
-        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (t0 + t < t1 && !(seq && seq[t0 + t] < 0)) {
-          const Quad q = *reinterpret_cast<const Quad*>(src + (t0 + t) * ld + n);
-          f = make_float4(to_f(q.v[0]), to_f(q.v[1]), to_f(q.v[2]), to_f(q.v[3]));
-        }
-        *reinterpret_cast<float4*>(dst + i * 4) = f;
-      }
-    }
-    return;
-  }
-  for (int i = threadIdx.x; i < TT * NP; i += THREADS) {
-    const int t = i / NP, n = i - t * NP;
-    dst[i] = t0 + t < t1 && n < N && !(seq && seq[t0 + t] < 0) ? to_f(src[(t0 + t) * ld + n]) : 0.f;
-  }
+  Rows<T, NP, TT, THREADS> r;
+  r.fetch(threadIdx.x, src, ld, t0, t1, seq, quads);
+  r.put(threadIdx.x, dst, src, ld, t0, t1, N, seq, quads);
 }
 
 // Two adjacent channels of an activation. `both`: one access for the two, where every row has
@@ -213,11 +232,6 @@ __device__ __forceinline__ float2 softplus2(float2 x) {
 }
 // x sigmoid(x)
 __device__ __forceinline__ float2 silu2(float2 x) { return __fmul2_rn(x, sigmoid2(x)); }
-// max |x| that keeps a NaN (as integer bits it is above all numbers)
-__device__ __forceinline__ unsigned max_bits(unsigned m, float2 x) {
-  return max(m, max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu));
-}
-
 // NPT states as pairs, and a tile row's values for them.
 template <int NPT>
 struct Pairs {
@@ -267,44 +281,30 @@ __device__ __forceinline__ float2 state_sums(const float* y) {
   return r;
 }
 
-// 2^x for the products x = dt A2 of a pair of states. The special-function unit gives 16 an SM
-// and clock, the fused multiply-add pipes stand half idle beside it, so a part of the pairs
-// goes there: x = k + f, 2^f = 1 + f q(f) with q of degree 4 (relative error 1.2e-7, and that
-// of a rounding near 1, where decays act longest), k into the exponent. That form holds for
-// |x| < 126 only; kernels look at a tile's largest |dt| times the largest |A2| first.
-constexpr float kPolyRange = 126.f;
-__device__ __forceinline__ float2 pow2_poly(float2 dt, float2 A2) {
-  const float2 magic = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23: the sum's low bits are k
-  const float2 xi = __ffma2_rn(dt, A2, magic);
-  const float2 k = __fadd2_rn(xi, make_float2(-12582912.f, -12582912.f));
-  const float2 f = __ffma2_rn(dt, A2, make_float2(-k.x, -k.y));
-  float2 q = __ffma2_rn(f, make_float2(0.0013405575882643461f, 0.0013405575882643461f),
-                        make_float2(0.009670727886259556f, 0.009670727886259556f));
-  q = __ffma2_rn(f, q, make_float2(0.05550314858555794f, 0.05550314858555794f));
-  q = __ffma2_rn(f, q, make_float2(0.24022258818149567f, 0.24022258818149567f));
-  q = __ffma2_rn(f, q, make_float2(0.6931471824645996f, 0.6931471824645996f));
-  q = __ffma2_rn(f, q, make_float2(1.f, 1.f));
-  return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(xi.x) << 23)),
-                     __int_as_float(__float_as_int(q.y) + (__float_as_int(xi.y) << 23)));
-}
-__device__ __forceinline__ float2 pow2_unit(float2 dt, float2 A2) {
-  const float2 x = __fmul2_rn(dt, A2);
+// exp(dt A) of a pair of states, A2 = A log2(e). The unit's 2^x cuts its argument off: for
+// arguments of -0.5 to -0.001 its results were 0.3 * 2^-24 too small on average, which a state
+// that is kept for a thousand tokens multiplies. Half a step of 2^-24 on the argument brings
+// the average to 0.05 * 2^-24 and costs nothing (a fused multiply-add for a product); a step
+// size of zero still gives exactly 1.
+__device__ __forceinline__ float2 decay(float2 dt, float2 A2) {
+  const float2 x = __ffma2_rn(dt, A2, all2(2.9802322387695312e-8f));
   return make_float2(ex2(x.x), ex2(x.y));
-}
-
-// The largest |x| of a CTA as integer bits: per warp, for a tile's readers.
-template <int WARPS>
-__device__ __forceinline__ float max_of(const unsigned (&m)[WARPS]) {
-  unsigned v = m[0];
-#pragma unroll
-  for (int k = 1; k < WARPS; ++k) v = max(v, m[k]);
-  return __uint_as_float(v);
 }
 
 // Start, end and membership of the tile's tokens as bit masks (at most 32 tokens).
 struct SeqMask {
   unsigned start, end, in;
 };
+template <int TT>
+__device__ __forceinline__ SeqMask warp_masks(const int* seq, int t0, int t1, int T) {
+  const int t = t0 + (threadIdx.x & 31);
+  const bool on = (threadIdx.x & 31) < TT && t < t1;
+  SeqMask m;
+  m.start = __ballot_sync(0xffffffffu, on && seq_starts(seq, t));
+  m.end = __ballot_sync(0xffffffffu, on && seq_ends(seq, t, T));
+  m.in = __ballot_sync(0xffffffffu, on && seq[t] >= 0);
+  return m;
+}
 __device__ __forceinline__ bool in_sequence(const int* seq, int t) { return !seq || seq[t] >= 0; }
 template <int TT>
 __device__ __forceinline__ void stage_masks(SeqMask* m, const int* seq, int t0, int t1, int T) {

@@ -1,11 +1,14 @@
 // Selective state space scan, forward: prompts, packed prompts and the training forward, and
 // the single-token step. The recurrence is in selective_scan.cuh.
 //
-// A channel's N states are split over LN threads, NPT in each, and stay in registers while the
-// CTA walks the time axis tile by tile: a tile's step sizes and inputs are worked out once per
-// (token, channel) into shared memory, then every thread runs its states through the tile's
-// tokens, then the threads add the partial outputs of their channel, apply the skip and the
-// gate and write. One exponential per (token, channel, state) is what bounds it.
+// A channel's N states are split over LN threads, NPT in each and two channels a thread, and
+// stay in registers while the CTA walks the time axis tile by tile: a tile's step sizes and
+// inputs are worked out once per (token, channel) into shared memory, then every thread runs
+// its states through the tile's tokens, then the partial outputs of a channel's threads are
+// added, the skip and the gate applied and the result written. One exponential per (token,
+// channel, state) is what bounds it, and next to that the shared-memory reads, whose cost is
+// bytes per thread whether or not threads read the same: the second channel halves those of
+// B and C.
 //
 // With few channels in all, the time axis is split into pieces: a first pass finds each
 // piece's end state from zero and the sum of its step sizes (its whole decay is
@@ -18,213 +21,264 @@ namespace scan {
 
 template <int LN, int NPT>
 struct Fwd {
-  static constexpr int THREADS = 128, WARPS = THREADS / 32;
-  static constexpr int DT = THREADS / LN;            // channels of a CTA
+  static constexpr int HALF = 128;                   // threads of the recurrence; as many for the element-wise work
+  static constexpr int THREADS = 2 * HALF;
+  static constexpr int DT = 2 * HALF / LN;           // channels of a CTA
   static constexpr int NP = LN * NPT;                // states, padded
-  static constexpr int TT = LN >= 4 ? 32 : 8 * LN;   // tokens of a tile
+  static constexpr int TT = LN >= 4 ? 16 : 8;      // tokens of a tile
   static constexpr int RUN = 8;                      // tokens unrolled
-  static constexpr int TWOS = TT * DT / 2 / THREADS; // couples of channels of a thread, one token each
-  static constexpr int STEP = 2 * LN;                // tokens between them
-  struct Smem {
+  static constexpr int TWOS = TT / LN;               // couples of channels of a thread, one token each
+  static constexpr int STEP = LN;                    // tokens between them
+  static constexpr int YS = DT + (LN > 1 ? 32 / LN : 0);  // row of partial outputs, padded off bank conflicts
+  struct Tile {
     float B[TT * NP], C[TT * NP];
-    float4 d[TT * DT];      // step size twice, step size * input twice: operands of paired arithmetic
-    float y[TT * THREADS];  // partial outputs
-    unsigned dt_max[WARPS], A_max[WARPS];
-    SeqMask m;
+    float2 d[TT * DT];       // step size, step size * input
+    float y[TT * LN * YS];   // partial outputs
+  };
+  struct Smem {
+    Tile tile[2];
   };
 };
 
-// What a thread holds: channel d and states n0 .. in the recurrence; channels pd, pd + 1, and
-// tokens tq, tq + STEP, .. of a tile, in the element-wise passes.
+// A thread of the recurrence: states n0 .. of channels d, d + 1.
 template <int LN, int NPT>
 struct Lane {
-  int n0, cl, d, tq, pc, pd;
-  bool on, on0, on1;
+  int nl, n0, cl, d;
+  bool c0, c1;
   __device__ __forceinline__ Lane(const Params& p, const Where& w) {
-    using F = Fwd<LN, NPT>;
     const int tid = threadIdx.x;
-    n0 = tid % LN * NPT, cl = tid / LN;
-    pc = tid % (F::DT / 2) * 2, tq = tid / (F::DT / 2);
-    d = w.g * p.Dg + w.d0 + cl, pd = w.g * p.Dg + w.d0 + pc;
-    on = w.d0 + cl < p.Dg, on0 = w.d0 + pc < p.Dg, on1 = w.d0 + pc + 1 < p.Dg;
+    nl = tid % LN, n0 = nl * NPT, cl = tid / LN * 2;
+    d = w.g * p.Dg + w.d0 + cl;
+    c0 = w.d0 + cl < p.Dg, c1 = w.d0 + cl + 1 < p.Dg;
   }
 };
-// One token of the recurrence for NPT states; POLY: this token's share of the decays goes to
-// the multiply-add pipes (3 pairs in 8, see pow2_poly).
-template <int NPT, bool POLY>
-__device__ __forceinline__ void advance(Pairs<NPT>& h, const Pairs<NPT>& A2, const float4 dd, const float* Brow,
-                                        int t) {
-  const float2 dt = make_float2(dd.x, dd.y), dtu = make_float2(dd.z, dd.w);
-  const Pairs<NPT> B = row_pairs<NPT>(Brow);
+// A thread of the element-wise work: channels pd, pd + 1 at tokens tq, tq + STEP, .. of a tile.
+template <int LN, int NPT>
+struct Couple {
+  int tid, pc, tq, pd;
+  bool on0, on1;
+  __device__ __forceinline__ Couple(const Params& p, const Where& w) {
+    using F = Fwd<LN, NPT>;
+    tid = threadIdx.x - F::HALF;
+    pc = tid % (F::DT / 2) * 2, tq = tid / (F::DT / 2);
+    pd = w.g * p.Dg + w.d0 + pc;
+    on0 = w.d0 + pc < p.Dg, on1 = w.d0 + pc + 1 < p.Dg;
+  }
+};
+
+// The states of a thread's two channels.
+template <int NPT>
+struct Both {
+  Pairs<NPT> c[2];
+};
+template <int LN, int NPT>
+__device__ __forceinline__ Both<NPT> load_both(const float* base, const Lane<LN, NPT>& q, int N, bool on) {
+  Both<NPT> r;
+  float x[NPT];
+  load_states<NPT>(base, q.d, q.n0, N, on && q.c0, x);
+  r.c[0] = pairs_of<NPT>(x);
+  load_states<NPT>(base, q.d + 1, q.n0, N, on && q.c1, x);
+  r.c[1] = pairs_of<NPT>(x);
+  return r;
+}
+template <int LN, int NPT>
+__device__ __forceinline__ void store_both(float* base, const Lane<LN, NPT>& q, int N, bool on, const Both<NPT>& h) {
+  float x[NPT];
+  unpair(h.c[0], x);
+  store_states<NPT>(base, q.d, q.n0, N, on && q.c0, x);
+  unpair(h.c[1], x);
+  store_states<NPT>(base, q.d + 1, q.n0, N, on && q.c1, x);
+}
+// A2 = A log2(e)
+template <int LN, int NPT>
+__device__ __forceinline__ Both<NPT> load_decays(const Params& p, const Lane<LN, NPT>& q) {
+  Both<NPT> A2 = load_both(p.A, q, p.N, true);
 #pragma unroll
-  for (int j = 0; j < NPT / 2; ++j) {
-    const int k = (t * (NPT / 2) + j) % 8;
-    const float2 a = POLY && (k == 1 || k == 4 || k == 6) ? pow2_poly(dt, A2.v[j]) : pow2_unit(dt, A2.v[j]);
-    h.v[j] = __ffma2_rn(a, h.v[j], __fmul2_rn(dtu, B.v[j]));
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int j = 0; j < NPT / 2; ++j) A2.c[c].v[j] = __fmul2_rn(A2.c[c].v[j], all2(kLog2e));
+  return A2;
+}
+
+// The CTA's barrier for its two halves, which wait at places of their own in the code.
+__device__ __forceinline__ void tile_barrier() { asm volatile("barrier.sync 1, 256;" ::: "memory"); }
+
+// The recurrence over one tile, by the first half of the CTA. STATE: states only, no outputs;
+// REV: backwards, h = a (h + x R).
+template <int LN, int NPT, bool SEQ, bool STATE, bool REV>
+__device__ __forceinline__ void run_tile(const Params& p, const Where& w, const Lane<LN, NPT>& q,
+                                         typename Fwd<LN, NPT>::Tile& s, const Both<NPT>& A2, Both<NPT>& h,
+                                         int t0, int tend, const float* edge) {
+  using F = Fwd<LN, NPT>;
+  const long long DN = (long long)p.D * p.N;
+  constexpr int every = save_every_of(NPT);
+  SeqMask mask{};
+  if (SEQ) mask = warp_masks<F::TT>(p.seq, t0, tend, p.L);
+  const unsigned edges = REV ? mask.end : STATE ? mask.start : mask.start | mask.end;
+#pragma unroll 1
+  for (int r0 = 0; r0 < F::TT; r0 += F::RUN) {
+    const int r = REV ? F::TT - F::RUN - r0 : r0;
+    if (t0 + r >= tend) continue;
+    const auto tokens = [&](auto checks) {
+#pragma unroll
+      for (int k = 0; k < F::RUN; ++k) {
+        const int t = r + (REV ? F::RUN - 1 - k : k);
+        if constexpr (decltype(checks)::value) {
+          if (t0 + t >= tend) continue;
+        }
+        if (!STATE && k % every == 0 && p.hsave)
+          store_both(p.hsave + ((long long)w.row * p.nsave + (t0 + t) / every) * DN, q, p.N, true, h);
+        if constexpr (decltype(checks)::value && SEQ) {
+          if ((REV ? mask.end : mask.start) >> t & 1) {
+            const int sq = p.seq[t0 + t];
+            h = load_both(edge + sq * DN, q, p.N, sq >= 0 && edge);
+          }
+        }
+        const float4 d4 = *reinterpret_cast<const float4*>(&s.d[t * F::DT + q.cl]);
+        const Pairs<NPT> B2 = row_pairs<NPT>(s.B + t * F::NP + q.n0);
+        Pairs<NPT> C2;
+        if (!STATE) C2 = row_pairs<NPT>(s.C + t * F::NP + q.n0);
+        float2 y = all2(0.f);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float2 dt = all2(c ? d4.z : d4.x), x = all2(c ? d4.w : d4.y);
+          float2 sum = all2(0.f);
+#pragma unroll
+          for (int j = 0; j < NPT / 2; ++j) {
+            const float2 a = decay(dt, A2.c[c].v[j]);
+            float2& hj = h.c[c].v[j];
+            if constexpr (REV) hj = __fmul2_rn(a, __ffma2_rn(x, B2.v[j], hj));
+            else hj = __ffma2_rn(a, hj, __fmul2_rn(x, B2.v[j]));
+            if (!STATE) sum = j ? __ffma2_rn(hj, C2.v[j], sum) : __fmul2_rn(hj, C2.v[j]);
+          }
+          (c ? y.y : y.x) = sum.x + sum.y;
+        }
+        if (!STATE) *reinterpret_cast<float2*>(&s.y[(t * LN + q.nl) * F::YS + q.cl]) = y;
+        if constexpr (decltype(checks)::value && SEQ && !STATE) {
+          if (p.fin && (mask.end >> t & 1)) {
+            const int sq = p.seq[t0 + t];
+            store_both(p.fin + sq * DN, q, p.N, sq >= 0, h);
+          }
+        }
+      }
+    };
+    if (t0 + r + F::RUN > tend || (SEQ && (edges >> r & 0xff))) tokens(std::true_type{});
+    else tokens(std::false_type{});
   }
 }
 
+// The first half of the CTA runs tile i while the second finishes the outputs of tile i - 1 and
+// prepares tile i + 1 in the other buffer; one barrier a tile.
 template <typename T, int LN, int NPT, bool SEQ>
-__global__ void __launch_bounds__(128) scan_fwd_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(256, NPT == 4 ? 3 : 1) scan_fwd_kernel(const __grid_constant__ Params p) {
   using F = Fwd<LN, NPT>;
   extern __shared__ __align__(16) unsigned char raw_smem[];
   auto& s = *reinterpret_cast<typename F::Smem*>(raw_smem);
   const Where w = where<F::DT>(p);
-  const Lane<LN, NPT> q(p, w);
-  const int tid = threadIdx.x;
   const int tbeg = w.piece * p.chunk, tend = min(p.L, tbeg + p.chunk);
+  const int ntiles = (tend - tbeg + F::TT - 1) / F::TT;
   const long long DN = (long long)p.D * p.N;
-  const int* seq = SEQ ? p.seq : nullptr;
 
-  float hs[NPT];
-  load_states<NPT>(p.A, q.d, q.n0, p.N, q.on, hs);
-  unsigned am = 0;
-#pragma unroll
-  for (int i = 0; i < NPT; i += 2) {
-    hs[i] *= kLog2e, hs[i + 1] *= kLog2e;
-    am = max_bits(am, make_float2(hs[i], hs[i + 1]));
+  if (threadIdx.x < F::HALF) {
+    const Lane<LN, NPT> q(p, w);
+    const Both<NPT> A2 = load_decays(p, q);
+    Both<NPT> h = p.nchunks > 1 ? load_both(p.cstate + ((long long)w.row * p.nchunks + w.piece) * DN, q, p.N, true)
+                                : load_both(p.init + w.row * DN, q, p.N, p.init && !SEQ);
+    for (int i = 0; i < ntiles; ++i) {
+      tile_barrier();
+      run_tile<LN, NPT, SEQ, false, false>(p, w, q, s.tile[i & 1], A2, h, tbeg + i * F::TT, tend, p.init);
+    }
+    tile_barrier();
+    if (!SEQ && p.fin && tend == p.L) store_both(p.fin + w.row * DN, q, p.N, true, h);
+    return;
   }
-  am = __reduce_max_sync(0xffffffffu, am);
-  if (tid % 32 == 0) s.A_max[tid / 32] = am;
-  const Pairs<NPT> A2 = pairs_of<NPT>(hs);
-  if (p.nchunks > 1)
-    load_states<NPT>(p.cstate + ((long long)w.row * p.nchunks + w.piece) * DN, q.d, q.n0, p.N, q.on, hs);
-  else
-    load_states<NPT>(p.init + w.row * DN, q.d, q.n0, p.N, q.on && p.init && !SEQ, hs);
-  Pairs<NPT> h = pairs_of<NPT>(hs);
+
+  const Couple<LN, NPT> q(p, w);
+  const int* seq = SEQ ? p.seq : nullptr;
   const float2 skip = params_of(p.Dskip, q.pd, q.on0, q.on1), bias = params_of(p.bias, q.pd, q.on0, q.on1);
-  const long long first = tbeg + q.tq;
-  const T* u = static_cast<const T*>(p.u) + w.row * p.u_b + first * p.u_l + q.pd;
-  const T* delta = static_cast<const T*>(p.delta) + w.row * p.delta_b + first * p.delta_l + q.pd;
-  const T* z = static_cast<const T*>(p.z) + w.row * p.z_b + first * p.z_l + q.pd;
+  const T* u = static_cast<const T*>(p.u) + w.row * p.u_b + q.pd;
+  const T* delta = static_cast<const T*>(p.delta) + w.row * p.delta_b + q.pd;
+  const T* z = static_cast<const T*>(p.z) + w.row * p.z_b + q.pd;
   const T* B = static_cast<const T*>(p.B) + w.row * p.B_b + w.g * p.B_g;
   const T* C = static_cast<const T*>(p.C) + w.row * p.C_b + w.g * p.C_g;
-  T* out = static_cast<T*>(p.out) + ((long long)w.row * p.L + first) * p.D + q.pd;
-  const long long u_step = F::STEP * p.u_l, delta_step = F::STEP * p.delta_l, z_step = F::STEP * p.z_l;
-  const long long out_step = (long long)F::STEP * p.D;
-  const int every = 32 / NPT;
-
-  for (int t0 = tbeg; t0 < tend; t0 += F::TT) {
-    Two<T> uu[F::TWOS], zz[F::TWOS], dd[F::TWOS];
-    if (SEQ) stage_masks<F::TT>(&s.m, p.seq, t0, tend, p.L);
+  T* out = static_cast<T*>(p.out) + (long long)w.row * p.L * p.D + q.pd;
+  // inputs and gates of the tile that is prepared, the one that runs and the one before
+  Two<T> u2[F::TWOS], z2[F::TWOS], u1[F::TWOS], z1[F::TWOS], u0[F::TWOS], z0[F::TWOS], dd[F::TWOS];
+  Rows<T, F::NP, F::TT, F::HALF> rB, rC;
+  for (int i = -1; i <= ntiles; ++i) {
+    const int tn = tbeg + (i + 1) * F::TT, tl = tbeg + (i - 1) * F::TT;
+    if (i + 1 < ntiles) {
 #pragma unroll
-    for (int k = 0; k < F::TWOS; ++k) {
-      const int tok = t0 + q.tq + k * F::STEP;
-      const bool in = tok < tend && in_sequence(seq, tok), on0 = in && q.on0, on1 = in && q.on1;
-      dd[k] = load_two(delta, on0, on1, p.couples), uu[k] = load_two(u, on0, on1, p.couples);
-      zz[k] = load_two(z, on0 && p.z, on1 && p.z, p.couples);
-      delta += delta_step, u += u_step, z += z_step;
-    }
-    stage_rows<T, F::NP, F::TT, F::THREADS>(s.B, B, p.B_l, t0, tend, p.N, seq, p.quads);
-    stage_rows<T, F::NP, F::TT, F::THREADS>(s.C, C, p.C_l, t0, tend, p.N, seq, p.quads);
-    unsigned m = 0;
-#pragma unroll
-    for (int k = 0; k < F::TWOS; ++k) {
-      const int t = q.tq + k * F::STEP, tok = t0 + t;
-      float2 dt = __fadd2_rn(two_f(dd[k]), bias);
-      if (p.softplus) dt = softplus2(dt);
-      if (!(tok < tend && in_sequence(seq, tok))) dt = all2(0.f);
-      const float2 x = __fmul2_rn(dt, two_f(uu[k]));
-      m = max_bits(m, dt);
-      s.d[t * F::DT + q.pc] = make_float4(dt.x, dt.x, x.x, x.x);
-      s.d[t * F::DT + q.pc + 1] = make_float4(dt.y, dt.y, x.y, x.y);
-    }
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (tid % 32 == 0) s.dt_max[tid / 32] = m;
-    __syncthreads();
-    const bool poly = max_of(s.dt_max) * max_of(s.A_max) < kPolyRange;
-
-#pragma unroll 1
-    for (int r = 0; r < F::TT && t0 + r < tend; r += F::RUN) {
-      if (p.hsave && (t0 + r) % every == 0) {
-        unpair(h, hs);
-        store_states<NPT>(p.hsave + ((long long)w.row * p.nsave + (t0 + r) / every) * DN, q.d, q.n0, p.N, q.on, hs);
+      for (int k = 0; k < F::TWOS; ++k) {
+        const int tok = tn + q.tq + k * F::STEP;
+        const bool in = tok < tend && in_sequence(seq, tok), on0 = in && q.on0, on1 = in && q.on1;
+        dd[k] = load_two(delta + tok * p.delta_l, on0, on1, p.couples), u2[k] = load_two(u + tok * p.u_l, on0, on1, p.couples);
+        z2[k] = load_two(z + tok * p.z_l, on0 && p.z, on1 && p.z, p.couples);
       }
-      const bool slow =
-          t0 + r + F::RUN > tend || (SEQ && ((s.m.start | s.m.end) >> r & 0xff)) || (p.hsave && every < F::RUN);
-      const auto tokens = [&](auto use_poly, auto checks) {
-#pragma unroll
-        for (int k = 0; k < F::RUN; ++k) {
-          const int t = r + k;
-          if constexpr (decltype(checks)::value) {
-            if (t0 + t >= tend) break;
-            if (p.hsave && k && (t0 + t) % every == 0) {
-              unpair(h, hs);
-              store_states<NPT>(p.hsave + ((long long)w.row * p.nsave + (t0 + t) / every) * DN, q.d, q.n0, p.N, q.on,
-                                hs);
-            }
-            if (SEQ && (s.m.start >> t & 1)) {
-              const int sq = p.seq[t0 + t];
-              load_states<NPT>(p.init + sq * DN, q.d, q.n0, p.N, q.on && sq >= 0 && p.init, hs);
-              h = pairs_of<NPT>(hs);
-            }
-          }
-          advance<NPT, decltype(use_poly)::value>(h, A2, s.d[t * F::DT + q.cl], s.B + t * F::NP + q.n0, k);
-          const Pairs<NPT> C2 = row_pairs<NPT>(s.C + t * F::NP + q.n0);
-          float2 y = __fmul2_rn(h.v[0], C2.v[0]);
-#pragma unroll
-          for (int j = 1; j < NPT / 2; ++j) y = __ffma2_rn(h.v[j], C2.v[j], y);
-          s.y[t * F::THREADS + tid] = y.x + y.y;
-          if constexpr (decltype(checks)::value) {
-            if (SEQ && p.fin && (s.m.end >> t & 1)) {
-              const int sq = p.seq[t0 + t];
-              unpair(h, hs);
-              store_states<NPT>(p.fin + sq * DN, q.d, q.n0, p.N, q.on && sq >= 0, hs);
-            }
-          }
-        }
-      };
-      if (slow) tokens(std::false_type{}, std::true_type{});
-      else if (poly) tokens(std::true_type{}, std::false_type{});
-      else tokens(std::false_type{}, std::false_type{});
+      rB.fetch(q.tid, B, p.B_l, tn, tend, seq, p.quads), rC.fetch(q.tid, C, p.C_l, tn, tend, seq, p.quads);
     }
-    __syncthreads();
-
+    if (i >= 1) {
+      const auto& tile = s.tile[(i - 1) & 1];
 #pragma unroll
-    for (int k = 0; k < F::TWOS; ++k) {
-      const int t = q.tq + k * F::STEP, tok = t0 + t;
-      float2 y = __ffma2_rn(skip, two_f(uu[k]), state_sums<LN>(s.y + t * F::THREADS + q.pc * LN));
-      if (p.z) y = __fmul2_rn(y, silu2(two_f(zz[k])));
-      if (SEQ && !(s.m.in >> t & 1)) y = all2(0.f);  // a token of no sequence
-      store_two(out, y, q.on0 && tok < tend, q.on1 && tok < tend, p.couples);
-      out += out_step;
+      for (int k = 0; k < F::TWOS; ++k) {
+        const int t = q.tq + k * F::STEP, tok = tl + t;
+        float2 y = __fmul2_rn(skip, two_f(u0[k]));
+#pragma unroll
+        for (int j = 0; j < LN; ++j)
+          y = __fadd2_rn(y, *reinterpret_cast<const float2*>(&tile.y[(t * LN + j) * F::YS + q.pc]));
+        if (p.z) y = __fmul2_rn(y, silu2(two_f(z0[k])));
+        if (SEQ && tok < tend && seq[tok] < 0) y = all2(0.f);  // a token of no sequence
+        store_two(out + (long long)tok * p.D, y, q.on0 && tok < tend, q.on1 && tok < tend, p.couples);
+      }
     }
-    if (SEQ) __syncthreads();  // the masks are written again
-  }
-  if (!SEQ && p.fin && tend == p.L) {
-    unpair(h, hs);
-    store_states<NPT>(p.fin + w.row * DN, q.d, q.n0, p.N, q.on, hs);
+    if (i + 1 < ntiles) {
+      auto& tile = s.tile[(i + 1) & 1];
+#pragma unroll
+      for (int k = 0; k < F::TWOS; ++k) {
+        const int t = q.tq + k * F::STEP, tok = tn + t;
+        float2 dt = __fadd2_rn(two_f(dd[k]), bias);
+        if (p.softplus) dt = softplus2(dt);
+        if (!(tok < tend && in_sequence(seq, tok))) dt = all2(0.f);
+        const float2 x = __fmul2_rn(dt, two_f(u2[k]));
+        *reinterpret_cast<float4*>(&tile.d[t * F::DT + q.pc]) = make_float4(dt.x, x.x, dt.y, x.y);
+      }
+      rB.put(q.tid, tile.B, B, p.B_l, tn, tend, p.N, seq, p.quads);
+      rC.put(q.tid, tile.C, C, p.C_l, tn, tend, p.N, seq, p.quads);
+    }
+#pragma unroll
+    for (int k = 0; k < F::TWOS; ++k) u0[k] = u1[k], z0[k] = z1[k], u1[k] = u2[k], z1[k] = z2[k];
+    if (i < ntiles) tile_barrier();
   }
 }
 
 // A piece's end state from zero (REV: the carry that leaves its first token from zero at its
 // last), and the sum of its step sizes.
 template <typename T, int LN, int NPT, bool REV, bool SEQ>
-__global__ void __launch_bounds__(128) scan_chunk_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(256, NPT == 4 ? 3 : 1) scan_chunk_kernel(const __grid_constant__ Params p) {
   using F = Fwd<LN, NPT>;
   extern __shared__ __align__(16) unsigned char raw_smem[];
   auto& s = *reinterpret_cast<typename F::Smem*>(raw_smem);
   const Where w = where<F::DT>(p);
-  const Lane<LN, NPT> q(p, w);
-  const int tid = threadIdx.x;
   const int tbeg = w.piece * p.chunk, tend = min(p.L, tbeg + p.chunk);
-  const long long DN = (long long)p.D * p.N;
-  const int* seq = SEQ ? p.seq : nullptr;
+  const int ntiles = (tend - tbeg + F::TT - 1) / F::TT;
+  const long long DN = (long long)p.D * p.N, at = (long long)w.row * p.nchunks + w.piece;
+  const auto tile_at = [&](int i) { return tbeg + (REV ? ntiles - 1 - i : i) * F::TT; };
 
-  float hs[NPT], sum = 0.f;
-  load_states<NPT>(p.A, q.d, q.n0, p.N, q.on, hs);
-  unsigned am = 0;
-#pragma unroll
-  for (int i = 0; i < NPT; i += 2) {
-    hs[i] *= kLog2e, hs[i + 1] *= kLog2e;
-    am = max_bits(am, make_float2(hs[i], hs[i + 1]));
+  if (threadIdx.x < F::HALF) {
+    const Lane<LN, NPT> q(p, w);
+    const Both<NPT> A2 = load_decays(p, q);
+    Both<NPT> h = load_both(p.A, q, p.N, false);
+    for (int i = 0; i < ntiles; ++i) {
+      tile_barrier();
+      run_tile<LN, NPT, SEQ, true, REV>(p, w, q, s.tile[i & 1], A2, h, tile_at(i), tend, REV ? p.dfin : p.init);
+    }
+    store_both(p.cstate + at * DN, q, p.N, true, h);
+    tile_barrier();
+    return;
   }
-  am = __reduce_max_sync(0xffffffffu, am);
-  if (tid % 32 == 0) s.A_max[tid / 32] = am;
-  const Pairs<NPT> A2 = pairs_of<NPT>(hs);
-  Pairs<NPT> h;
-#pragma unroll
-  for (int j = 0; j < NPT / 2; ++j) h.v[j] = make_float2(0.f, 0.f);
+
+  const Couple<LN, NPT> q(p, w);
+  const int* seq = SEQ ? p.seq : nullptr;
   const float2 bias = params_of(p.bias, q.pd, q.on0, q.on1);
   const T* delta = static_cast<const T*>(p.delta) + w.row * p.delta_b + q.pd;
   // what drives the recurrence: u and B, or dout (gated) and C
@@ -235,84 +289,47 @@ __global__ void __launch_bounds__(128) scan_chunk_kernel(const __grid_constant__
   const T* R = REV ? static_cast<const T*>(p.C) + w.row * p.C_b + w.g * p.C_g
                    : static_cast<const T*>(p.B) + w.row * p.B_b + w.g * p.B_g;
   const long long r_l = REV ? p.C_l : p.B_l;
-  const float* edge = REV ? p.dfin : p.init;
-
-  const int ntiles = (tend - tbeg + F::TT - 1) / F::TT;
-  for (int k0 = 0; k0 < ntiles; ++k0) {
-    const int t0 = tbeg + (REV ? ntiles - 1 - k0 : k0) * F::TT;
-    if (SEQ) stage_masks<F::TT>(&s.m, p.seq, t0, tend, p.L);
-    Two<T> dd[F::TWOS], vv[F::TWOS], zz[F::TWOS];
+  float2 sum = all2(0.f);
+  for (int i = -1; i < ntiles; ++i) {
+    if (i + 1 < ntiles) {
+      const int tn = tile_at(i + 1);
+      auto& tile = s.tile[(i + 1) & 1];
+      Two<T> dd[F::TWOS], vv[F::TWOS], zz[F::TWOS];
+      Rows<T, F::NP, F::TT, F::HALF> rows;
 #pragma unroll
-    for (int k = 0; k < F::TWOS; ++k) {
-      const int tok = t0 + q.tq + k * F::STEP;
-      const bool in = tok < tend && in_sequence(seq, tok), on0 = in && q.on0, on1 = in && q.on1;
-      dd[k] = load_two(delta + tok * p.delta_l, on0, on1, p.couples);
-      vv[k] = load_two(v + tok * v_l, on0, on1, p.couples);
-      if (REV) zz[k] = load_two(z + tok * p.z_l, on0 && p.z, on1 && p.z, p.couples);
+      for (int k = 0; k < F::TWOS; ++k) {
+        const int tok = tn + q.tq + k * F::STEP;
+        const bool in = tok < tend && in_sequence(seq, tok), on0 = in && q.on0, on1 = in && q.on1;
+        dd[k] = load_two(delta + tok * p.delta_l, on0, on1, p.couples);
+        vv[k] = load_two(v + tok * v_l, on0, on1, p.couples);
+        if (REV) zz[k] = load_two(z + tok * p.z_l, on0 && p.z, on1 && p.z, p.couples);
+      }
+      rows.fetch(q.tid, R, r_l, tn, tend, seq, p.quads);
+#pragma unroll
+      for (int k = 0; k < F::TWOS; ++k) {
+        const int t = q.tq + k * F::STEP, tok = tn + t;
+        float2 dt = __fadd2_rn(two_f(dd[k]), bias), x = two_f(vv[k]);
+        if (p.softplus) dt = softplus2(dt);
+        if (!(tok < tend && in_sequence(seq, tok))) dt = all2(0.f);
+        if (REV && p.z) x = __fmul2_rn(x, silu2(two_f(zz[k])));
+        if (!REV) x = __fmul2_rn(x, dt);
+        sum = __fadd2_rn(sum, dt);
+        *reinterpret_cast<float4*>(&tile.d[t * F::DT + q.pc]) = make_float4(dt.x, x.x, dt.y, x.y);
+      }
+      rows.put(q.tid, tile.B, R, r_l, tn, tend, p.N, seq, p.quads);
     }
-    stage_rows<T, F::NP, F::TT, F::THREADS>(s.B, R, r_l, t0, tend, p.N, seq, p.quads);
-    unsigned m = 0;
-#pragma unroll
-    for (int k = 0; k < F::TWOS; ++k) {
-      const int t = q.tq + k * F::STEP, tok = t0 + t;
-      float2 dt = __fadd2_rn(two_f(dd[k]), bias), x = two_f(vv[k]);
-      if (p.softplus) dt = softplus2(dt);
-      if (!(tok < tend && in_sequence(seq, tok))) dt = all2(0.f);
-      if (REV && p.z) x = __fmul2_rn(x, silu2(two_f(zz[k])));
-      if (!REV) x = __fmul2_rn(x, dt);
-      m = max_bits(m, dt);
-      s.d[t * F::DT + q.pc] = make_float4(dt.x, dt.x, x.x, x.x);
-      s.d[t * F::DT + q.pc + 1] = make_float4(dt.y, dt.y, x.y, x.y);
-    }
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (tid % 32 == 0) s.dt_max[tid / 32] = m;
-    __syncthreads();
-    const bool poly = max_of(s.dt_max) * max_of(s.A_max) < kPolyRange;
-
-#pragma unroll 1
-    for (int r0 = 0; r0 < F::TT; r0 += F::RUN) {
-      const int r = REV ? F::TT - F::RUN - r0 : r0;
-      if (t0 + r >= tend) continue;
-      const auto tokens = [&](auto use_poly, auto checks) {
-#pragma unroll
-        for (int k = 0; k < F::RUN; ++k) {
-          const int t = r + (REV ? F::RUN - 1 - k : k);
-          if constexpr (decltype(checks)::value) {
-            if (t0 + t >= tend) continue;
-            if (SEQ && ((REV ? s.m.end : s.m.start) >> t & 1)) {
-              const int sq = p.seq[t0 + t];
-              load_states<NPT>(edge + sq * DN, q.d, q.n0, p.N, q.on && sq >= 0 && edge, hs);
-              h = pairs_of<NPT>(hs);
-            }
-          }
-          const float4 dd4 = s.d[t * F::DT + q.cl];
-          const float* row = s.B + t * F::NP + q.n0;
-          sum += dd4.x;
-          if constexpr (REV) {
-            const Pairs<NPT> R2 = row_pairs<NPT>(row);
-            const float2 dt = make_float2(dd4.x, dd4.y), x = make_float2(dd4.z, dd4.w);
-#pragma unroll
-            for (int j = 0; j < NPT / 2; ++j) {
-              const int i = (k * (NPT / 2) + j) % 8;
-              const float2 a = decltype(use_poly)::value && (i == 1 || i == 4 || i == 6) ? pow2_poly(dt, A2.v[j])
-                                                                                         : pow2_unit(dt, A2.v[j]);
-              h.v[j] = __fmul2_rn(a, __ffma2_rn(x, R2.v[j], h.v[j]));
-            }
-          } else {
-            advance<NPT, decltype(use_poly)::value>(h, A2, dd4, row, k);
-          }
-        }
-      };
-      if (t0 + r + F::RUN > tend || (SEQ && ((REV ? s.m.end : s.m.start) >> r & 0xff))) tokens(std::false_type{}, std::true_type{});
-      else if (poly) tokens(std::true_type{}, std::false_type{});
-      else tokens(std::false_type{}, std::false_type{});
-    }
-    __syncthreads();
+    if (i + 1 < ntiles) tile_barrier();
   }
-  const long long at = (long long)w.row * p.nchunks + w.piece;
-  unpair(h, hs);
-  store_states<NPT>(p.cstate + at * DN, q.d, q.n0, p.N, q.on, hs);
-  if (q.on && tid % LN == 0) p.csum[at * p.D + q.d] = sum;
+  // the couples' threads have the step sizes' sums, one token in STEP each
+  float* part = s.tile[0].y;
+  *reinterpret_cast<float2*>(&part[q.tq * F::DT + q.pc]) = sum;
+  tile_barrier();
+  if (q.tq == 0) {
+#pragma unroll
+    for (int j = 1; j < F::STEP; ++j) sum = __fadd2_rn(sum, *reinterpret_cast<const float2*>(&part[j * F::DT + q.pc]));
+    if (q.on0) p.csum[at * p.D + q.pd] = sum.x;
+    if (q.on1) p.csum[at * p.D + q.pd + 1] = sum.y;
+  }
 }
 
 // Turns the pieces' end states into the states that enter them, in place. One thread per

@@ -26,7 +26,7 @@ struct Bwd {
   static constexpr int THREADS = 256, WARPS = THREADS / 32;
   static constexpr int DT = THREADS / LN;     // channels of a CTA
   static constexpr int NP = LN * NPT;         // states, padded
-  static constexpr int SUB = 32 / NPT;        // tokens whose states are in registers: save_every()
+  static constexpr int SUB = save_every_of(NPT);  // tokens whose states are in registers: save_every()
   static constexpr int TB = 2 * SUB;          // tokens of a tile
   static constexpr int CG = 8 / LN;           // groups of 4 channels in a warp
   static constexpr int TS = LN < SUB ? LN : SUB;  // tokens side by side in a product's columns
@@ -40,7 +40,6 @@ struct Bwd {
     float s3[TB * THREADS];
     float dB[WARPS * CG][TB * NP], dC[WARPS * CG][TB * NP];
     float2 red[THREADS];
-    unsigned dt_max[WARPS], A_max[WARPS];
     SeqMask m;
   };
 };
@@ -97,14 +96,8 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
 
   float hs[NPT];
   load_states<NPT>(p.A, d, n0, p.N, on, hs);
-  unsigned am = 0;
 #pragma unroll
-  for (int i = 0; i < NPT; i += 2) {
-    hs[i] *= kLog2e, hs[i + 1] *= kLog2e;
-    am = max_bits(am, make_float2(hs[i], hs[i + 1]));
-  }
-  am = __reduce_max_sync(0xffffffffu, am);
-  if (lane == 0) s.A_max[warp] = am;
+  for (int i = 0; i < NPT; ++i) hs[i] *= kLog2e;
   const Pairs<NPT> A2 = pairs_of<NPT>(hs);
   if (p.nchunks > 1)
     load_states<NPT>(p.cstate + ((long long)w.row * p.nchunks + w.piece) * DN, d, n0, p.N, on, hs);
@@ -143,7 +136,6 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
       load_states<NPT>(kept + (2 * tile + half) * DN, d, n0, p.N, on && t0 + half * F::SUB < tend, h_kept[half]);
     stage_rows<T, F::NP, F::TB, F::THREADS>(s.B, B, p.B_l, t0, tend, p.N, seq, p.quads);
     stage_rows<T, F::NP, F::TB, F::THREADS>(s.C, C, p.C_l, t0, tend, p.N, seq, p.quads);
-    unsigned m = 0;
 #pragma unroll
     for (int k = 0; k < F::TWOS; ++k) {
       const int t = tq + k * F::STEP, tok = t0 + t;
@@ -153,21 +145,17 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
         if (!(tok < tend && in_sequence(seq, tok))) dt = all2(0.f);
         const float2 x = __fmul2_rn(dt, two_f(uu[k]));
         if (p.z) dy = __fmul2_rn(dy, silu2(two_f(zz[k])));
-        m = max_bits(m, dt);
         s.d[t * F::DT + pc] = make_float4(dt.x, dt.x, x.x, x.x), s.d[t * F::DT + pc + 1] = make_float4(dt.y, dt.y, x.y, x.y);
         *reinterpret_cast<float4*>(&s.dy[t * F::DT + pc]) = make_float4(dy.x, dy.x, dy.y, dy.y);
       }
     }
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (lane == 0) s.dt_max[warp] = m;
     __syncthreads();
-    const bool poly = max_of(s.dt_max) * max_of(s.A_max) < kPolyRange;
 
 #pragma unroll 1
     for (int half = 1; half >= 0; --half) {
       const int b = half * F::SUB;
       if (t0 + b >= tend) continue;
-      const auto tokens = [&](auto use_poly, auto checks) {
+      const auto tokens = [&](auto checks) {
         float2 a[F::SUB][H], ah[F::SUB][H];
         Pairs<NPT> h;
 #pragma unroll
@@ -188,8 +176,7 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
           const Pairs<NPT> B2 = row_pairs<NPT>(s.B + t * F::NP + n0);
 #pragma unroll
           for (int j = 0; j < H; ++j) {
-            const int i = (k * H + j) % 8;
-            a[k][j] = decltype(use_poly)::value && (i == 1 || i == 5) ? pow2_poly(dt, A2.v[j]) : pow2_unit(dt, A2.v[j]);
+            a[k][j] = decay(dt, A2.v[j]);
             ah[k][j] = __fmul2_rn(a[k][j], h.v[j]);
             h.v[j] = __ffma2_rn(dtu, B2.v[j], ah[k][j]);
           }
@@ -269,9 +256,8 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
         for (int j = 0; j < H; ++j) dA.v[j] = __fadd2_rn(dA.v[j], dA_here.v[j]);
       };
       if (t0 + b + F::SUB > tend || (SEQ && ((s.m.start | s.m.end) >> b & ((1u << F::SUB) - 1))))
-        tokens(std::false_type{}, std::true_type{});
-      else if (poly) tokens(std::true_type{}, std::false_type{});
-      else tokens(std::false_type{}, std::false_type{});
+        tokens(std::true_type{});
+      else tokens(std::false_type{});
     }
     __syncthreads();
 
