@@ -57,7 +57,7 @@ inline Shape shape_of(int N) {
   return {8, 16};
 }
 // Tokens between two saved states: those whose states the backward kernel holds in registers.
-__host__ __device__ constexpr int save_every_of(int NPT) { return NPT == 4 ? 4 : 32 / NPT; }
+__host__ __device__ constexpr int save_every_of(int NPT) { return NPT == 16 ? 2 : 4; }
 inline int save_every(int N) { return save_every_of(shape_of(N).NPT); }
 
 
@@ -248,6 +248,29 @@ template <int NPT>
 __device__ __forceinline__ void unpair(const Pairs<NPT>& x, float (&y)[NPT]) {
 #pragma unroll
   for (int j = 0; j < NPT / 2; ++j) y[2 * j] = x.v[j].x, y[2 * j + 1] = x.v[j].y;
+}
+// The states of a thread's two channels, d and d + 1.
+template <int NPT>
+struct Both {
+  Pairs<NPT> c[2];
+};
+template <int NPT>
+__device__ __forceinline__ Both<NPT> load_both(const float* base, int d, int n0, int N, bool on0, bool on1) {
+  Both<NPT> r;
+  float x[NPT];
+  load_states<NPT>(base, d, n0, N, on0, x);
+  r.c[0] = pairs_of<NPT>(x);
+  load_states<NPT>(base, d + 1, n0, N, on1, x);
+  r.c[1] = pairs_of<NPT>(x);
+  return r;
+}
+template <int NPT>
+__device__ __forceinline__ void store_both(float* base, int d, int n0, int N, bool on0, bool on1, const Both<NPT>& h) {
+  float x[NPT];
+  unpair(h.c[0], x);
+  store_states<NPT>(base, d, n0, N, on0, x);
+  unpair(h.c[1], x);
+  store_states<NPT>(base, d + 1, n0, N, on1, x);
 }
 template <int NPT>
 __device__ __forceinline__ Pairs<NPT> row_pairs(const float* row) {  // 16-byte aligned

@@ -66,28 +66,13 @@ struct Couple {
   }
 };
 
-// The states of a thread's two channels.
-template <int NPT>
-struct Both {
-  Pairs<NPT> c[2];
-};
 template <int LN, int NPT>
 __device__ __forceinline__ Both<NPT> load_both(const float* base, const Lane<LN, NPT>& q, int N, bool on) {
-  Both<NPT> r;
-  float x[NPT];
-  load_states<NPT>(base, q.d, q.n0, N, on && q.c0, x);
-  r.c[0] = pairs_of<NPT>(x);
-  load_states<NPT>(base, q.d + 1, q.n0, N, on && q.c1, x);
-  r.c[1] = pairs_of<NPT>(x);
-  return r;
+  return load_both<NPT>(base, q.d, q.n0, N, on && q.c0, on && q.c1);
 }
 template <int LN, int NPT>
 __device__ __forceinline__ void store_both(float* base, const Lane<LN, NPT>& q, int N, bool on, const Both<NPT>& h) {
-  float x[NPT];
-  unpair(h.c[0], x);
-  store_states<NPT>(base, q.d, q.n0, N, on && q.c0, x);
-  unpair(h.c[1], x);
-  store_states<NPT>(base, q.d + 1, q.n0, N, on && q.c1, x);
+  store_both<NPT>(base, q.d, q.n0, N, on && q.c0, on && q.c1, h);
 }
 // A2 = A log2(e)
 template <int LN, int NPT>
