@@ -9,14 +9,14 @@
 // with the decays a and a h[t-1] held in registers, then g back through them, two channels a
 // thread. Meanwhile the second part finishes the element-wise gradients of the tile before and
 // prepares the step sizes and gates of the next (one barrier a tile). Sums over a channel's
-// states (s1, s2 and y) pass through shared memory. Sums over channels (dB, dC) are products of
-// the state matrix h (or g) of a token with its vector dy (or dt u), so the tensor cores take
-// them: one mma.sync of 16 states x 8 channels for a pair of states a thread, the vector in the
-// column of its token and zeros in the others. The factors have 11 bits there: for bf16 inputs
-// they are rounded to that (2^-11 each, against 2^-8 of dB's and dC's own type), for fp16 and
-// fp32 split in two such parts, three products a pair, 2^-21. What the CTAs of a group have of
-// dB and dC, and what the rows and pieces have of dA, dD and dbias, is written as partials and
-// added in a fixed order afterwards, so that results do not depend on timing.
+// states (s1, s2 and y) pass through shared memory. Sums over channels (dB, dC): a thread adds
+// its two channels' products, and the tensor cores add over the threads, as products of the
+// matrix of those (16 states x 4 threads, one mma.sync a pair of states) with a vector of ones
+// in the column of the token and zeros in the others. The matrix has 11 bits there: for bf16
+// inputs the products are rounded to that (2^-11, against 2^-8 of dB's and dC's own type), for
+// fp16 and fp32 split in two such parts, 2^-21. What the CTAs of a group have of dB and dC, and
+// what the rows and pieces have of dA, dD and dbias, is written as partials and added in a
+// fixed order afterwards, so that results do not depend on timing.
 #include "selective_scan.cuh"
 namespace ttt {
 namespace scan {
@@ -54,28 +54,26 @@ __device__ __forceinline__ float tf32(float x) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
   return __uint_as_float(r);
 }
-__device__ __forceinline__ void mma_16x8x8(float (&c)[4], float2 v0, float2 v1, float2 b) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(__float_as_uint(v0.x)), "r"(__float_as_uint(v0.y)), "r"(__float_as_uint(v1.x)),
-                 "r"(__float_as_uint(v1.y)), "r"(__float_as_uint(b.x)), "r"(__float_as_uint(b.y)));
+// c += A b for the 16 x 4 matrix A with this thread's a in rows lane / 4 and 8 + lane / 4.
+__device__ __forceinline__ void mma_16x8x4(float (&c)[4], float2 a, float b) {
+  asm("mma.sync.aligned.m16n8k4.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(__float_as_uint(a.x)), "r"(__float_as_uint(a.y)), "r"(__float_as_uint(b)));
 }
-__device__ __forceinline__ float2 tf32_2(float2 v) { return make_float2(tf32(v.x), tf32(v.y)); }
 // The 11 leading bits of x, for the split form: x = high + high(x - high) to 2^-21.
-__device__ __forceinline__ float high(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
-__device__ __forceinline__ float2 high2(float2 v) { return make_float2(high(v.x), high(v.y)); }
-__device__ __forceinline__ float2 low2(float2 v, float2 h) { return high2(__fadd2_rn(v, neg2(h))); }
-// c += v b over the warp's channels: v0, v1 a pair of states of the thread's two channels, b the
-// vector's values for two channels; SPLIT: both factors in two parts.
+__device__ __forceinline__ float2 high2(float2 v) {
+  return make_float2(__uint_as_float(__float_as_uint(v.x) & 0xffffe000u),
+                     __uint_as_float(__float_as_uint(v.y) & 0xffffe000u));
+}
+// Adds a pair of states' v over the 4 threads of a channel group to the column that `one` marks.
 template <bool SPLIT>
-__device__ __forceinline__ void add_product(float (&c)[4], float2 v0, float2 v1, float2 b, float2 b_low) {
+__device__ __forceinline__ void add_over_channels(float (&c)[4], float2 v, float one) {
   if constexpr (SPLIT) {
-    const float2 x = high2(v0), y = high2(v1);
-    mma_16x8x8(c, low2(v0, x), low2(v1, y), b);
-    mma_16x8x8(c, x, y, b_low);
-    mma_16x8x8(c, x, y, b);
+    const float2 h = high2(v);
+    mma_16x8x4(c, high2(__fadd2_rn(v, neg2(h))), one);
+    mma_16x8x4(c, h, one);
   } else {
-    mma_16x8x8(c, tf32_2(v0), tf32_2(v1), b);
+    mma_16x8x4(c, make_float2(tf32(v.x), tf32(v.y)), one);
   }
 }
 
@@ -100,12 +98,11 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
 
   if (threadIdx.x < F::MAIN) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // lane -> states and channels, as the products' first operand wants them: rows lane / 4 are
-    // (channel group, state run), columns lane % 4 and 4 + lane % 4 two channels of the group
+    // lane -> states and channels, as the sums over channels want them: rows lane / 4 of the
+    // matrix are (channel group, state run), columns lane % 4 the two channels' threads
     const int l3 = lane & 3, row8 = lane >> 2, cg = row8 / LN, nl = row8 % LN, n0 = nl * NPT;
     const int cl = warp * F::CW + 8 * cg + 2 * l3;
-    // and as the second operand wants them: column lane / 4 is (token, channel group)
-    const int col_tok = row8 / F::CG, col_ch = warp * F::CW + 8 * (row8 % F::CG) + 2 * l3;
+    const int col_tok = row8 / F::CG;  // and the token of this thread's column of the sums
     const int d = w.g * p.Dg + w.d0 + cl;
     const bool c0 = w.d0 + cl < p.Dg, c1 = w.d0 + cl + 1 < p.Dg;
     const float* kept = p.hsave + (long long)w.row * p.nsave * DN;
@@ -206,14 +203,6 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
           for (int j = 0; j < H; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) accB[j][e] = accC[j][e] = 0.f;
-          float2 vB = all2(0.f), vC = vB;  // the products' vectors, in this lane's token and channels
-          if (col_tok < TS) {
-            const float4 d4 = *reinterpret_cast<const float4*>(&tile.d[(b + g0 + col_tok) * F::DT + col_ch]);
-            vB = make_float2(d4.y, d4.w);
-            vC = *reinterpret_cast<const float2*>(&tile.dy[(b + g0 + col_tok) * F::DT + col_ch]);
-          }
-          const float2 hB = SPLIT ? high2(vB) : tf32_2(vB), hC = SPLIT ? high2(vC) : tf32_2(vC);
-          const float2 lB = SPLIT ? low2(vB, hB) : all2(0.f), lC = SPLIT ? low2(vC, hC) : all2(0.f);
 #pragma unroll
           for (int k = g0 + TS - 1; k >= g0; --k) {
             if constexpr (CHECK) {
@@ -226,9 +215,8 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
             const float4 d4 = *reinterpret_cast<const float4*>(&tile.d[(b + k) * F::DT + cl]);
             const float2 dy2 = *reinterpret_cast<const float2*>(&tile.dy[(b + k) * F::DT + cl]);
             const Pairs<NPT> B2 = row_pairs<NPT>(tile.B + (b + k) * F::NP + n0), C2 = row_pairs<NPT>(tile.C + (b + k) * F::NP + n0);
-            const bool mine = col_tok == k - g0;
-            const float2 zero = all2(0.f), bB = mine ? hB : zero, bC = mine ? hC : zero;
-            const float2 eB = SPLIT && mine ? lB : zero, eC = SPLIT && mine ? lC : zero;
+            const float one = col_tok == k - g0 ? 1.f : 0.f;
+            const float2 zero = all2(0.f);
             float2 s1[2] = {zero, zero}, s2[2] = {zero, zero}, s3[2] = {zero, zero};
 #pragma unroll
             for (int j = 0; j < H; ++j) {
@@ -245,8 +233,8 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
                 dA.c[c].v[j] = __ffma2_rn(q, all2(c ? d4.z : d4.x), dA.c[c].v[j]);
                 carry.c[c].v[j] = __fmul2_rn(a[k][c][j], g[c]);
               }
-              add_product<SPLIT>(accB[j], g[0], g[1], bB, eB);
-              add_product<SPLIT>(accC[j], hn[0], hn[1], bC, eC);
+              add_over_channels<SPLIT>(accB[j], __ffma2_rn(g[0], all2(d4.y), __fmul2_rn(g[1], all2(d4.w))), one);
+              add_over_channels<SPLIT>(accC[j], __ffma2_rn(hn[0], all2(dy2.x), __fmul2_rn(hn[1], all2(dy2.y))), one);
             }
             const int o = ((b + k) * LN + nl) * F::YS + cl;
             *reinterpret_cast<float2*>(&tile.s1[o]) = make_float2(s1[0].x + s1[0].y, s1[1].x + s1[1].y);
