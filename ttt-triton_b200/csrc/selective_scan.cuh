@@ -344,11 +344,13 @@ __device__ __forceinline__ void stage_masks(SeqMask* m, const int* seq, int t0, 
 // Launches the pass over pieces (local end states, then the states entering each piece), when
 // the time axis is split. REV: the backward recurrence's carries instead of the states.
 int chunk_states(const Params& p, int dt, bool rev, cudaStream_t st, const char* who);
-// Splits the time axis and lays its part of the scratch out behind `extra` bytes of the caller.
-int plan(Params& p, void* scratch, size_t scratch_bytes, size_t extra, const char* who);
+// How the time axis is split, the scratch that takes (bytes), and its place behind `extra`
+// bytes of the caller's.
+void plan_pieces(Params& p, bool backward);
+size_t piece_bytes(const Params& p);
+int plan_scratch(Params& p, void* scratch, size_t scratch_bytes, size_t extra, const char* who);
 bool quads(const Params& p, int dt);
 bool couples(const Params& p, int dt);
-size_t plan_bytes(int rows, int L, int D, int N);
 int check_sizes(const char* who, int rows, int L, int D, int G, int N, int dt);
 
 template <typename F>

@@ -324,23 +324,32 @@ __global__ void __launch_bounds__(256) scan_carry_kernel(const __grid_constant__
   const long long DN = (long long)p.D * p.N, i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= DN * p.rows) return;
   const int row = i / DN;
-  const long long e = i - row * DN;
-  const int d = e / p.N;
-  const float A2 = p.A[e] * kLog2e;
+  const long long i_dn = i - row * DN;
+  const int d = i_dn / p.N;
+  const float A2 = p.A[i_dn] * kLog2e;
   const float* edge = REV ? p.dfin : p.init;
-  float h = edge && !p.seq ? edge[row * DN + e] : 0.f;
-  for (int k = 0; k < p.nchunks; ++k) {
-    const int c = REV ? p.nchunks - 1 - k : k;
-    const long long at = (long long)row * p.nchunks + c;
-    bool cut = false;
-    if (p.seq) {  // a sequence that starts (ends) in the piece cuts what follows off from what came before
-      const int t0 = c * p.chunk, t1 = min(p.L, t0 + p.chunk);
-      cut = REV ? t1 >= p.L || p.seq[t1] != p.seq[t0] : t0 == 0 || p.seq[t0 - 1] != p.seq[t1 - 1];
+  float h = edge && !p.seq ? edge[row * DN + i_dn] : 0.f;
+  constexpr int AHEAD = 8;  // pieces read together: the chain through them is a few cycles each
+  for (int k0 = 0; k0 < p.nchunks; k0 += AHEAD) {
+    float own[AHEAD], sum[AHEAD];
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e) {
+      if (k0 + e >= p.nchunks) break;
+      const long long at = (long long)row * p.nchunks + (REV ? p.nchunks - 1 - k0 - e : k0 + e);
+      own[e] = p.cstate[at * DN + i_dn], sum[e] = p.csum[at * p.D + d];
     }
-    float* q = p.cstate + at * DN + e;
-    const float own = *q;
-    *q = h;
-    h = cut ? own : fmaf(ex2(A2 * p.csum[at * p.D + d]), h, own);
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e) {
+      if (k0 + e >= p.nchunks) break;
+      const int c = REV ? p.nchunks - 1 - k0 - e : k0 + e;
+      bool cut = false;
+      if (p.seq) {  // a sequence that starts (ends) in the piece cuts what follows off from what came before
+        const int t0 = c * p.chunk, t1 = min(p.L, t0 + p.chunk);
+        cut = REV ? t1 >= p.L || p.seq[t1] != p.seq[t0] : t0 == 0 || p.seq[t0 - 1] != p.seq[t1 - 1];
+      }
+      p.cstate[((long long)row * p.nchunks + c) * DN + i_dn] = h;
+      h = cut ? own[e] : fmaf(ex2(A2 * sum[e]), h, own[e]);
+    }
   }
 }
 
@@ -482,18 +491,29 @@ bool couples(const Params& p, int dt) {
   return true;
 }
 
-// Pieces of the time axis: as many as bring the device about two full waves of warps, no
-// piece under 64 tokens.
-int pieces(int rows, int L, int D, int N) {
-  const Shape s = shape_of(N);
-  const long long warps = ((long long)rows * D * s.LN + 31) / 32, want = (long long)sm_count() * 32;
-  if (warps >= want / 2 || L < 256) return 1;
-  long long n = (want + warps - 1) / warps;
-  if (n > L / 64) n = L / 64;
-  return n < 1 ? 1 : (int)n;
+// Tokens of a piece of the time axis, a multiple of 64 (tiles and kept states of every shape
+// start on it), or L for one piece. Splitting costs a pass over the pieces first, `extra` of the
+// main pass's time, about 128 tokens' worth of launches and 3 a piece; it pays where the `blocks` CTAs of
+// whole rows leave SMs empty, or a last round of them nearly so. An SM runs `resident` CTAs at
+// once; k of them take 0.4 + 0.6 k / resident of that time. Measured, 16 x 2048 x 1536 states
+// of 16: backward 1.32 ms whole (384 CTAs on 296 places), EEE in 3 pieces; forward prompt of
+// 1 x 8192 x 1024: FFF whole, GGG in 26 pieces.
+int piece_tokens(long long blocks, int L, int resident, float extra) {
+  const long long sms = sm_count(), places = sms * resident;
+  float best = 0.f;
+  int tokens = L;
+  const long long most = L / 64 < 1024 ? L / 64 : 1024;
+  for (long long n = 1; n <= (most > 1 ? most : 1); ++n) {
+    const int len = n == 1 ? L : (int)(((L + n - 1) / n + 63) / 64 * 64);
+    const long long all = blocks * ((L + len - 1) / len), rest = all % places;
+    float rounds = (float)(all / places);
+    if (rest) rounds += 0.4f + 0.6f * (float)((rest + sms - 1) / sms) / resident;
+    const float cost = n == 1 ? rounds * L : rounds * len * (1.f + extra) + 128.f + 3.f * n;
+    if (n == 1 || cost < best) best = cost, tokens = len;
+    if (all > 8 * places) break;
+  }
+  return tokens;
 }
-// Tokens of a piece: a multiple of 64, so that tiles and saved states of every shape start on it.
-int piece_tokens(int L, int n) { return ((L + n - 1) / n + 63) / 64 * 64; }
 
 int check_sizes(const char* who, int rows, int L, int D, int G, int N, int dt) {
   TTT_REQUIRE(rows >= 1 && L >= 1 && D >= 1 && G >= 1 && N >= 1, TTT_ERR_SHAPE,
@@ -507,26 +527,29 @@ int check_sizes(const char* who, int rows, int L, int D, int G, int N, int dt) {
   return TTT_OK;
 }
 
-// Splits the time axis and lays the scratch out; `extra` bytes of the caller come first.
-int plan(Params& p, void* scratch, size_t scratch_bytes, size_t extra, const char* who) {
-  const int n = pieces(p.rows, p.L, p.D, p.N);
-  p.chunk = n > 1 ? piece_tokens(p.L, n) : p.L;
+// How the time axis is split, forwards or backwards: the CTAs have the same channels.
+static int split(int rows, int L, int D, int G, int N, bool backward) {
+  const int DT = 256 / shape_of(N).LN;
+  const long long blocks = (long long)rows * G * ((D / G + DT - 1) / DT);
+  const bool narrow = shape_of(N).NPT == 4;
+  return backward ? piece_tokens(blocks, L, narrow ? 2 : 1, 0.3f) : piece_tokens(blocks, L, narrow ? 3 : 1, 0.5f);
+}
+void plan_pieces(Params& p, bool backward) {
+  p.chunk = split(p.rows, p.L, p.D, p.G, p.N, backward);
   p.nchunks = (p.L + p.chunk - 1) / p.chunk;
-  const size_t states = (size_t)p.rows * p.nchunks * p.D;
-  const size_t need = extra + (p.nchunks > 1 ? states * (p.N + 1) * sizeof(float) : 0);
+}
+size_t piece_bytes(const Params& p) {
+  return p.nchunks > 1 ? (size_t)p.rows * p.nchunks * p.D * (p.N + 1) * sizeof(float) : 0;
+}
+int plan_scratch(Params& p, void* scratch, size_t scratch_bytes, size_t extra, const char* who) {
+  const size_t need = extra + piece_bytes(p);
   TTT_REQUIRE(!need || (scratch && scratch_bytes >= need), TTT_ERR_SCRATCH, "%s: scratch of %zu bytes needed, got %zu",
               who, need, scratch ? scratch_bytes : (size_t)0);
   if (p.nchunks > 1) {
     p.cstate = reinterpret_cast<float*>(static_cast<char*>(scratch) + extra);
-    p.csum = p.cstate + states * p.N;
+    p.csum = p.cstate + (size_t)p.rows * p.nchunks * p.D * p.N;
   }
   return TTT_OK;
-}
-size_t plan_bytes(int rows, int L, int D, int N) {
-  const int n = pieces(rows, L, D, N);
-  if (n <= 1) return 0;
-  const int chunk = piece_tokens(L, n), nchunks = (L + chunk - 1) / chunk;
-  return nchunks > 1 ? (size_t)rows * nchunks * D * (N + 1) * sizeof(float) : 0;
 }
 
 }  // namespace scan
@@ -535,8 +558,11 @@ size_t plan_bytes(int rows, int L, int D, int N) {
 using namespace ttt;
 
 extern "C" size_t ttt_selective_scan_fwd_scratch_bytes(int rows, int L, int D, int G, int N) {
-  if (rows < 1 || L < 1 || D < 1 || G < 1 || N < 1 || N > scan::kMaxStates) return 0;
-  return scan::plan_bytes(rows, L, D, N);
+  if (rows < 1 || L < 1 || D < 1 || G < 1 || N < 1 || N > scan::kMaxStates || D % G) return 0;
+  scan::Params p{};
+  p.rows = rows, p.L = L, p.D = D, p.G = G, p.N = N;
+  scan::plan_pieces(p, false);
+  return scan::piece_bytes(p);
 }
 
 extern "C" size_t ttt_selective_scan_saved_bytes(int rows, int L, int D, int N) {
@@ -566,7 +592,8 @@ extern "C" int ttt_selective_scan_fwd(int rows, int L, int D, int G, int N, cons
   const int every = scan::save_every(N);
   p.nsave = (L + every - 1) / every;
   p.quads = scan::quads(p, dt), p.couples = scan::couples(p, dt);
-  if ((rc = scan::plan(p, scratch, scratch_bytes, 0, who))) return rc;
+  scan::plan_pieces(p, false);
+  if ((rc = scan::plan_scratch(p, scratch, scratch_bytes, 0, who))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (p.nchunks > 1 && (rc = scan::chunk_states(p, dt, false, st, who))) return rc;
   return dt == DT_BF16  ? scan::launch_fwd<__nv_bfloat16>(p, st, who)

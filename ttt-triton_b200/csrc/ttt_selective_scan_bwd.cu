@@ -498,18 +498,13 @@ static int launch_bwd(Params p, void* dB, void* dC, float* dparams, cudaStream_t
 
 using namespace ttt;
 
-static int bwd_pieces(int rows, int L, int D, int N) {
-  scan::Params p{};
-  p.rows = rows, p.L = L, p.D = D, p.N = N;
-  char dummy;
-  scan::plan(p, &dummy, ~(size_t)0, 0, "");
-  return p.nchunks;
-}
-
 extern "C" size_t ttt_selective_scan_bwd_scratch_bytes(int rows, int L, int D, int G, int N) {
   if (rows < 1 || L < 1 || D < 1 || G < 1 || N < 1 || N > scan::kMaxStates || D % G) return 0;
-  const scan::BwdScratch s = scan::bwd_scratch(rows, L, D, G, N, bwd_pieces(rows, L, D, N));
-  return 2 * s.part_bc + s.part_p + scan::plan_bytes(rows, L, D, N);
+  scan::Params p{};
+  p.rows = rows, p.L = L, p.D = D, p.G = G, p.N = N;
+  scan::plan_pieces(p, true);
+  const scan::BwdScratch s = scan::bwd_scratch(rows, L, D, G, N, p.nchunks);
+  return 2 * s.part_bc + s.part_p + scan::piece_bytes(p);
 }
 
 extern "C" int ttt_selective_scan_bwd(int rows, int L, int D, int G, int N, const void* u, const void* delta,
@@ -537,9 +532,9 @@ extern "C" int ttt_selective_scan_bwd(int rows, int L, int D, int G, int N, cons
   const int every = scan::save_every(N);
   p.nsave = (L + every - 1) / every;
   p.quads = scan::quads(p, dt), p.couples = scan::couples(p, dt);
-  const int nchunks = bwd_pieces(rows, L, D, N);
-  const scan::BwdScratch s = scan::bwd_scratch(rows, L, D, G, N, nchunks);
-  if ((rc = scan::plan(p, scratch, scratch_bytes, 2 * s.part_bc + s.part_p, who))) return rc;
+  scan::plan_pieces(p, true);
+  const scan::BwdScratch s = scan::bwd_scratch(rows, L, D, G, N, p.nchunks);
+  if ((rc = scan::plan_scratch(p, scratch, scratch_bytes, 2 * s.part_bc + s.part_p, who))) return rc;
   p.tiles = (int)s.tiles;
   p.part_B = static_cast<float*>(scratch);
   p.part_C = p.part_B + s.part_bc / sizeof(float);
