@@ -12,9 +12,22 @@ import ctypes
 import torch
 
 from _core import _on_tensor_device
-from _lib import check, dtype_code, lib, ptr, require_cuda, stream_of
+from _lib import check, dtype_code, lib, require_cuda
 
 MAX_STATES = 128
+
+
+# These calls are short: for a single token the host's work is most of their time. Addresses go
+# to ctypes as plain integers, and the current stream is asked for without wrapping it.
+_current_stream = torch._C._cuda_getCurrentRawStream
+
+
+def ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def stream_of(t):
+    return _current_stream(t.device.index)
 
 
 def _rows(t):
@@ -39,7 +52,7 @@ def _same(ref, **tensors):
 
 
 def _shaped(name, t, shape):
-    if t is not None and tuple(t.shape) != tuple(shape):
+    if t is not None and t.shape != shape:
         raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
 
 
@@ -66,7 +79,7 @@ def packed(cu_seqlens, x):
 
 # --------------------------------------------------------------------------- selective scan
 def check_scan(u, delta, A, B, C, D, z, delta_bias, init, nseq):
-    require_cuda(*(t for t in (u, delta, A, B, C, D, z, delta_bias, init) if t is not None))
+    require_cuda(*[t for t in (u, delta, A, B, C, D, z, delta_bias, init) if t is not None])
     dtype_code(u)
     if u.dim() != 3:
         raise ValueError(f"u must be [B, L, D], got shape {tuple(u.shape)}")
@@ -131,9 +144,9 @@ def selective_scan_backward(u, delta, A, B, C, D, z, delta_bias, softplus, init,
     rows, L, W = u.shape
     G, N = B.shape[2], A.shape[1]
     dev, dt = u.device, u.dtype
-    du, ddelta = (torch.empty(rows, L, W, device=dev, dtype=dt) for _ in range(2))
-    dz = torch.empty(rows, L, W, device=dev, dtype=dt) if z is not None else None
-    dB, dC = (torch.empty(rows, L, G, N, device=dev, dtype=dt) for _ in range(2))
+    du, ddelta = torch.empty_like(dout), torch.empty_like(dout)
+    dz = torch.empty_like(dout) if z is not None else None
+    dB, dC = torch.empty(2, rows, L, G, N, device=dev, dtype=dt).unbind(0)
     dinit = None
     if want_dinit:
         dinit = dfin.clone() if dfin is not None else torch.zeros(init.shape, device=dev, dtype=torch.float32)
@@ -171,7 +184,7 @@ def _check_step(state, index, rows, inputs, shape):
 def selective_scan_step(state, u, delta, A, B, C, D, z, delta_bias, softplus, index):
     """One token per row: out [B, D]; state [slots, D, N] fp32 updated in place."""
     inputs = (state, u, delta, A, B, C, D, z, delta_bias)
-    require_cuda(*(t for t in (*inputs, index) if t is not None))
+    require_cuda(*[t for t in (*inputs, index) if t is not None])
     if u.dim() != 2:
         raise ValueError(f"u must be [B, D], got shape {tuple(u.shape)}")
     rows, W = u.shape

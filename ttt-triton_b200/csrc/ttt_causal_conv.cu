@@ -41,38 +41,78 @@ template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
 };
+// VEC channels' values as pairs (the last one's second is unused where VEC is 1).
+template <int VEC>
+struct Vals {
+  static constexpr int H = (VEC + 1) / 2;
+  float2 v[H];
+};
 template <typename T, int VEC>
-__device__ __forceinline__ Pack<T, VEC> zero_pack() {
-  Pack<T, VEC> r;
+__device__ __forceinline__ Vals<VEC> unpack(const Pack<T, VEC>& r) {
+  Vals<VEC> x;
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) r.v[e] = from_f<T>(0.f);
-  return r;
+  for (int j = 0; j < Vals<VEC>::H; ++j)
+    x.v[j] = make_float2(to_f(r.v[2 * j]), 2 * j + 1 < VEC ? to_f(r.v[(2 * j + 1) % VEC]) : 0.f);
+  return x;
+}
+template <int VEC>
+__device__ __forceinline__ Vals<VEC> zeros() {
+  Vals<VEC> x;
+#pragma unroll
+  for (int j = 0; j < Vals<VEC>::H; ++j) x.v[j] = make_float2(0.f, 0.f);
+  return x;
 }
 template <typename T, int VEC>
 __device__ __forceinline__ Pack<T, VEC> load(const void* base, long long at) {
   return *reinterpret_cast<const Pack<T, VEC>*>(static_cast<const T*>(base) + at);
 }
 template <typename T, int VEC>
-__device__ __forceinline__ void store(void* base, long long at, const float (&x)[VEC]) {
+__device__ __forceinline__ void store(void* base, long long at, const Vals<VEC>& x) {
   Pack<T, VEC> r;
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) r.v[e] = from_f<T>(x[e]);
+  for (int e = 0; e < VEC; ++e) r.v[e] = from_f<T>(e % 2 ? x.v[e / 2].y : x.v[e / 2].x);
   *reinterpret_cast<Pack<T, VEC>*>(static_cast<T*>(base) + at) = r;
 }
+template <int VEC>
+__device__ __forceinline__ Vals<VEC> fma_of(const Vals<VEC>& a, const Vals<VEC>& b, const Vals<VEC>& c) {
+  Vals<VEC> r;
+#pragma unroll
+  for (int j = 0; j < Vals<VEC>::H; ++j) r.v[j] = __ffma2_rn(a.v[j], b.v[j], c.v[j]);
+  return r;
+}
+__device__ __forceinline__ float2 sigmoid2(float2 x) {
+  const float2 m = __fmul2_rn(x, make_float2(-scan::kLog2e, -scan::kLog2e));
+  const float2 e = __fadd2_rn(make_float2(scan::ex2(m.x), scan::ex2(m.y)), make_float2(1.f, 1.f));
+  return make_float2(scan::rcp(e.x), scan::rcp(e.y));
+}
 
-// The channels' weights, tap 0 on the oldest row.
+// The channels' weights, tap 0 on the oldest row, and bias.
 template <int K, int VEC>
 struct Taps {
-  float w[K][VEC], b[VEC];
-  __device__ __forceinline__ Taps(const Params& p, int d, bool on) {
+  Vals<VEC> w[K], b;
+  __device__ __forceinline__ Taps(const Params& p, int d) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
+    for (int j = 0; j < Vals<VEC>::H; ++j) {
+      const int d0 = d + 2 * j, d1 = d + (2 * j + 1 < VEC ? 2 * j + 1 : 2 * j);
 #pragma unroll
-      for (int k = 0; k < K; ++k) w[k][e] = on ? p.w[(long long)(d + e) * K + k] : 0.f;
-      b[e] = on && p.b ? p.b[d + e] : 0.f;
+      for (int k = 0; k < K; ++k) w[k].v[j] = make_float2(p.w[(long long)d0 * K + k], p.w[(long long)d1 * K + k]);
+      b.v[j] = make_float2(p.b ? p.b[d0] : 0.f, p.b ? p.b[d1] : 0.f);
     }
   }
+  // bias + sum of taps over x and the K - 1 rows before it, hist[0] the nearest
+  __device__ __forceinline__ Vals<VEC> at(const Vals<VEC>& x, const Vals<VEC> (&hist)[K - 1]) const {
+    Vals<VEC> q = fma_of(w[K - 1], x, b);
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) q = fma_of(w[K - 2 - j], hist[j], q);
+    return q;
+  }
 };
+template <int K, int VEC>
+__device__ __forceinline__ void push(Vals<VEC> (&hist)[K - 1], const Vals<VEC>& x) {
+#pragma unroll
+  for (int j = K - 2; j > 0; --j) hist[j] = hist[j - 1];
+  hist[0] = x;
+}
 
 struct At {
   int row, t0, t1;
@@ -86,148 +126,201 @@ __device__ __forceinline__ At run_of(const Params& p, long long id) {
   a.t1 = a.on ? min(p.L, a.t0 + p.run) : 0;
   return a;
 }
-__device__ __forceinline__ bool starts(const Params& p, int t) { return p.seq ? scan::seq_starts(p.seq, t) : t == 0; }
+template <bool SEQ>
+__device__ __forceinline__ bool starts(const Params& p, int t) {
+  return SEQ ? scan::seq_starts(p.seq, t) : t == 0;
+}
+template <bool SEQ>
 __device__ __forceinline__ bool ends(const Params& p, int t) {
-  return p.seq ? scan::seq_ends(p.seq, t, p.L) : t == p.L - 1;
+  return SEQ ? scan::seq_ends(p.seq, t, p.L) : t == p.L - 1;
+}
+// Whether none of the tokens t .. t + U - 1 starts or ends a sequence or belongs to none.
+template <int U, bool SEQ>
+__device__ __forceinline__ bool plain(const Params& p, int t) {
+  if (!SEQ) return t > 0 && t + U < p.L;
+  const int i = t + (threadIdx.x & 31);
+  const bool bad = (threadIdx.x & 31) < U && (i >= p.L || p.seq[i] < 0 || scan::seq_starts(p.seq, i) || scan::seq_ends(p.seq, i, p.L));
+  return !__any_sync(0xffffffffu, bad);
 }
 
-// The K - 1 rows before a sequence's first token: hist[0] is the nearest.
+// The K - 1 rows before a sequence's first token.
 template <typename T, int K, int VEC>
-__device__ __forceinline__ void initial_rows(const Params& p, int s, int d, float (&hist)[K - 1][VEC]) {
+__device__ __forceinline__ void initial_rows(const Params& p, int s, int d, Vals<VEC> (&hist)[K - 1]) {
 #pragma unroll
-  for (int j = 0; j < K - 1; ++j) {
-    Pack<T, VEC> r = zero_pack<T, VEC>();
-    if (p.init && s >= 0) r = load<T, VEC>(p.init, ((long long)s * (K - 1) + K - 2 - j) * p.D + d);
+  for (int j = 0; j < K - 1; ++j)
+    hist[j] = p.init && s >= 0 ? unpack<T, VEC>(load<T, VEC>(p.init, ((long long)s * (K - 1) + K - 2 - j) * p.D + d))
+                               : zeros<VEC>();
+}
+// The rows before token t0 > 0 of a run (of its sequence: `first` is its first token if that is
+// among them).
+template <typename T, int K, int VEC, bool SEQ>
+__device__ __forceinline__ void rows_before(const Params& p, const T* x, int t0, int d, int& first,
+                                            Vals<VEC> (&hist)[K - 1]) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) hist[j][e] = to_f(r.v[e]);
+  for (int j = 0; j < K - 1; ++j) hist[j] = zeros<VEC>();
+  for (int t = max(0, t0 - (K - 1)); t < t0; ++t) {
+    if (SEQ && starts<SEQ>(p, t)) initial_rows<T, K, VEC>(p, p.seq[t], d, hist), first = t;
+    push<K, VEC>(hist, unpack<T, VEC>(load<T, VEC>(x, t * p.x_l)));
   }
 }
 
-template <typename T, int K, int VEC>
+template <typename T, int K, int VEC, bool SEQ>
 __global__ void __launch_bounds__(kWarps * 32) conv_fwd_kernel(const __grid_constant__ Params p) {
   constexpr int U = 8;  // tokens loaded together
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = (p.D / VEC + 31) / 32;
   const long long blk = blockIdx.x / groups;
-  const int d = ((int)(blockIdx.x - blk * groups) * 32 + lane) * VEC;
+  int d = ((int)(blockIdx.x - blk * groups) * 32 + lane) * VEC;
   const At a = run_of(p, blk * kWarps + warp);
-  if (!a.on || d >= p.D) return;
-  const Taps<K, VEC> taps(p, d, true);
+  if (!a.on) return;
+  const bool on = d < p.D;
+  if (!on) d = 0;  // the lanes past the row stay for the warp's votes and write nothing
+  const Taps<K, VEC> taps(p, d);
   const T* x = static_cast<const T*>(p.x) + a.row * p.x_b + d;
-  float hist[K - 1][VEC] = {};
-  for (int t = max(0, a.t0 - (K - 1)); t < a.t1;) {
-    const int n = min(U, (t < a.t0 ? a.t0 : a.t1) - t);
-    Pack<T, VEC> in[U];
+  T* y = static_cast<T*>(p.y) + (long long)a.row * p.L * p.D + d;
+  Vals<VEC> hist[K - 1];
+  int first = 0;
+  rows_before<T, K, VEC, SEQ>(p, x, a.t0, d, first, hist);
+  const auto output = [&](const Vals<VEC>& v) {
+    Vals<VEC> q = taps.at(v, hist);
+    if (p.act)
 #pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (i < n) in[i] = load<T, VEC>(x, (t + i) * p.x_l);
+      for (int j = 0; j < Vals<VEC>::H; ++j) q.v[j] = __fmul2_rn(q.v[j], sigmoid2(q.v[j]));
+    push<K, VEC>(hist, v);
+    return q;
+  };
+  for (int t = a.t0; t < a.t1;) {
+    if (t + U <= a.t1 && plain<U, SEQ>(p, t)) {
+      Pack<T, VEC> in[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (i >= n) break;
-      const int tok = t + i, s = p.seq ? p.seq[tok] : a.row;
-      if (starts(p, tok)) initial_rows<T, K, VEC>(p, s, d, hist);
-      float v[VEC], y[VEC];
+      for (int i = 0; i < U; ++i) in[i] = load<T, VEC>(x, (t + i) * p.x_l);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        v[e] = to_f(in[i].v[e]);
-        float q = fmaf(taps.w[K - 1][e], v[e], taps.b[e]);
-#pragma unroll
-        for (int j = 0; j < K - 1; ++j) q = fmaf(taps.w[K - 2 - j][e], hist[j][e], q);
-        y[e] = s < 0 ? 0.f : p.act ? q * scan::sigmoid(q) : q;
-#pragma unroll
-        for (int j = K - 2; j > 0; --j) hist[j][e] = hist[j - 1][e];
-        hist[0][e] = v[e];
+      for (int i = 0; i < U; ++i) {
+        const Vals<VEC> q = output(unpack<T, VEC>(in[i]));
+        if (on) store<T, VEC>(y, (long long)(t + i) * p.D, q);
       }
-      if (tok >= a.t0) {
-        store<T, VEC>(p.y, ((long long)a.row * p.L + tok) * p.D + d, y);
-        if (p.fin && s >= 0 && ends(p, tok))
-#pragma unroll
-          for (int j = 0; j < K - 1; ++j)
-            store<T, VEC>(p.fin, ((long long)s * (K - 1) + K - 2 - j) * p.D + d, hist[j]);
-      }
+      t += U;
+      continue;
     }
-    t += n;
+    for (const int stop = min(t + U, a.t1); t < stop; ++t) {
+      const int s = SEQ ? p.seq[t] : a.row;
+      if (starts<SEQ>(p, t)) initial_rows<T, K, VEC>(p, s, d, hist);
+      Vals<VEC> q = output(unpack<T, VEC>(load<T, VEC>(x, t * p.x_l)));
+      if (s < 0) q = zeros<VEC>();
+      if (on) store<T, VEC>(y, (long long)t * p.D, q);
+      if (on && p.fin && s >= 0 && ends<SEQ>(p, t))
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) store<T, VEC>(p.fin, ((long long)s * (K - 1) + K - 2 - j) * p.D + d, hist[j]);
+    }
   }
 }
 
-template <typename T, int K, int VEC>
+template <typename T, int K, int VEC, bool SEQ>
 __global__ void __launch_bounds__(kWarps * 32) conv_bwd_kernel(const __grid_constant__ Params p) {
+  constexpr int U = VEC >= 4 ? 4 : 8;
   __shared__ float red[kWarps][32 * VEC];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = (p.D / VEC + 31) / 32;
   const long long blk = blockIdx.x / groups;
-  const int d0 = (int)(blockIdx.x - blk * groups) * 32 * VEC, d = d0 + lane * VEC;
+  const int d0 = (int)(blockIdx.x - blk * groups) * 32 * VEC;
+  int d = d0 + lane * VEC;
   const At a = run_of(p, blk * kWarps + warp);
-  float dw[K + 1][VEC] = {};  // the taps' gradients, then the bias's
-  if (a.on && d < p.D) {
-    const Taps<K, VEC> taps(p, d, true);
+  const bool on = d < p.D;
+  if (!on) d = 0;
+  Vals<VEC> dw[K + 1];  // the taps' gradients, then the bias's
+#pragma unroll
+  for (int k = 0; k <= K; ++k) dw[k] = zeros<VEC>();
+  if (a.on) {
+    const Taps<K, VEC> taps(p, d);
     const T* x = static_cast<const T*>(p.x) + a.row * p.x_b + d;
     const T* dy = static_cast<const T*>(p.dy) + (long long)a.row * p.L * p.D + d;
     T* dx = static_cast<T*>(p.dx) + (long long)a.row * p.L * p.D + d;
-    float hist[K - 1][VEC] = {}, acc[K][VEC] = {};  // acc[j]: the gradient of the row j before
+    Vals<VEC> hist[K - 1], acc[K];  // acc[j]: the gradient of the row j before
     int first = -K;  // the sequence's first token, or any earlier place
+    rows_before<T, K, VEC, SEQ>(p, x, a.t0, d, first, hist);
+#pragma unroll
+    for (int j = 0; j < K; ++j) acc[j] = zeros<VEC>();
     const int stop = min(p.L, a.t1 + K - 1);
+    // the token's gradient of p; `own`: its products are this run's
+    const auto token = [&](const Vals<VEC>& v, const Vals<VEC>& gy, bool own, bool none) {
+      Vals<VEC> g = gy;
+      if (p.act) {
+        const Vals<VEC> q = taps.at(v, hist);
+#pragma unroll
+        for (int j = 0; j < Vals<VEC>::H; ++j) {  // silu'(q) = s (1 + q (1 - s))
+          const float2 sg = sigmoid2(q.v[j]), one = make_float2(1.f, 1.f);
+          const float2 rest = __fadd2_rn(one, make_float2(-sg.x, -sg.y));
+          g.v[j] = __fmul2_rn(g.v[j], __fmul2_rn(sg, __ffma2_rn(q.v[j], rest, one)));
+        }
+      }
+      if (none) g = zeros<VEC>();  // a token of no sequence
+#pragma unroll
+      for (int j = 0; j < K; ++j) acc[j] = fma_of(taps.w[K - 1 - j], g, acc[j]);
+      if (own && !none) {
+        dw[K - 1] = fma_of(g, v, dw[K - 1]);
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) dw[K - 2 - j] = fma_of(g, hist[j], dw[K - 2 - j]);
+#pragma unroll
+        for (int j = 0; j < Vals<VEC>::H; ++j) dw[K].v[j] = __fadd2_rn(dw[K].v[j], g.v[j]);
+      }
+    };
+    const auto shift = [&](const Vals<VEC>& v) {
+#pragma unroll
+      for (int j = K - 1; j > 0; --j) acc[j] = acc[j - 1];
+      acc[0] = zeros<VEC>();
+      push<K, VEC>(hist, v);
+    };
     // row tok of the sequence (before `first`: of its initial state) has its whole gradient
-    const auto emit = [&](int tok, int s, const float (&g)[VEC]) {
+    const auto emit = [&](int tok, int s, const Vals<VEC>& g) {
       if (tok >= first) {
-        if (tok >= a.t0 && tok < a.t1) store<T, VEC>(dx, (long long)tok * p.D, g);
-      } else if (p.dinit && s >= 0 && first >= a.t0) {
+        if (on && tok >= a.t0 && tok < a.t1) store<T, VEC>(dx, (long long)tok * p.D, g);
+      } else if (on && p.dinit && s >= 0 && first >= a.t0) {
         store<T, VEC>(p.dinit, ((long long)s * (K - 1) + K - 1 + tok - first) * p.D + d, g);
       }
     };
-    for (int tok = max(0, a.t0 - (K - 1)); tok < stop; ++tok) {
-      const int s = p.seq ? p.seq[tok] : a.row;
-      if (starts(p, tok)) {
-        if (tok >= a.t1) break;
-        initial_rows<T, K, VEC>(p, s, d, hist);
-        first = tok;
+    bool done = false;
+    for (int t = a.t0; t < stop && !done;) {
+      // past the rows before the run, before its end, within a sequence
+      if (t >= max(a.t0, first) + K - 1 && t + U <= a.t1 && plain<U, SEQ>(p, t)) {
+        Pack<T, VEC> in[U], gy[U];
 #pragma unroll
-        for (int j = 0; j < K; ++j)
+        for (int i = 0; i < U; ++i)
+          in[i] = load<T, VEC>(x, (t + i) * p.x_l), gy[i] = load<T, VEC>(dy, (long long)(t + i) * p.D);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) acc[j][e] = 0.f;
-      }
-      const Pack<T, VEC> in = load<T, VEC>(x, tok * p.x_l);
-      float v[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = to_f(in.v[e]);
-      if (tok >= a.t0) {
-        const Pack<T, VEC> gy = load<T, VEC>(dy, (long long)tok * p.D);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          float q = fmaf(taps.w[K - 1][e], v[e], taps.b[e]);
-#pragma unroll
-          for (int j = 0; j < K - 1; ++j) q = fmaf(taps.w[K - 2 - j][e], hist[j][e], q);
-          float g = to_f(gy.v[e]);
-          if (p.act) g *= scan::silu_grad(q, scan::sigmoid(q));
-          if (s < 0) g = 0.f;  // a token of no sequence
-#pragma unroll
-          for (int j = 0; j < K; ++j) acc[j][e] = fmaf(taps.w[K - 1 - j][e], g, acc[j][e]);
-          if (tok < a.t1 && s >= 0) {
-            dw[K - 1][e] = fmaf(g, v[e], dw[K - 1][e]);
-#pragma unroll
-            for (int j = 0; j < K - 1; ++j) dw[K - 2 - j][e] = fmaf(g, hist[j][e], dw[K - 2 - j][e]);
-            dw[K][e] += g;
-          }
+        for (int i = 0; i < U; ++i) {
+          const Vals<VEC> v = unpack<T, VEC>(in[i]);
+          token(v, unpack<T, VEC>(gy[i]), true, false);
+          if (on) store<T, VEC>(dx, (long long)(t + i - (K - 1)) * p.D, acc[K - 1]);
+          shift(v);
         }
-        emit(tok - (K - 1), s, acc[K - 1]);
-        if (ends(p, tok)) {
+        t += U;
+        continue;
+      }
+      for (const int end = min(t + U, stop); t < end; ++t) {
+        const int s = SEQ ? p.seq[t] : a.row;
+        if (starts<SEQ>(p, t)) {
+          if (t >= a.t1) {
+            done = true;
+            break;
+          }
+          initial_rows<T, K, VEC>(p, s, d, hist);
+          first = t;
+#pragma unroll
+          for (int j = 0; j < K; ++j) acc[j] = zeros<VEC>();
+        }
+        const Vals<VEC> v = unpack<T, VEC>(load<T, VEC>(x, t * p.x_l));
+        token(v, unpack<T, VEC>(load<T, VEC>(dy, (long long)t * p.D)), t < a.t1, s < 0);
+        emit(t - (K - 1), s, acc[K - 1]);
+        if (ends<SEQ>(p, t)) {
 #pragma unroll
           for (int j = K - 2; j >= 0; --j) {
             if (p.dfin && s >= 0) {
-              const Pack<T, VEC> f = load<T, VEC>(p.dfin, ((long long)s * (K - 1) + K - 2 - j) * p.D + d);
+              const Vals<VEC> f = unpack<T, VEC>(load<T, VEC>(p.dfin, ((long long)s * (K - 1) + K - 2 - j) * p.D + d));
 #pragma unroll
-              for (int e = 0; e < VEC; ++e) acc[j][e] += to_f(f.v[e]);
+              for (int e = 0; e < Vals<VEC>::H; ++e) acc[j].v[e] = __fadd2_rn(acc[j].v[e], f.v[e]);
             }
-            emit(tok - j, s, acc[j]);
+            emit(t - j, s, acc[j]);
           }
         }
-      }
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-#pragma unroll
-        for (int j = K - 1; j > 0; --j) acc[j][e] = acc[j - 1][e];
-        acc[0][e] = 0.f;
-#pragma unroll
-        for (int j = K - 2; j > 0; --j) hist[j][e] = hist[j - 1][e];
-        hist[0][e] = v[e];
+        shift(v);
       }
     }
   }
@@ -236,7 +329,7 @@ __global__ void __launch_bounds__(kWarps * 32) conv_bwd_kernel(const __grid_cons
 #pragma unroll
   for (int k = 0; k <= K; ++k) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) red[warp][lane * VEC + e] = dw[k][e];
+    for (int e = 0; e < VEC; ++e) red[warp][lane * VEC + e] = e % 2 ? dw[k].v[e / 2].y : dw[k].v[e / 2].x;
     __syncthreads();
     for (int c = threadIdx.x; c < 32 * VEC; c += kWarps * 32) {
       if (d0 + c < p.D) {
@@ -321,8 +414,11 @@ template <typename T, int K, int VEC, bool BWD>
 static int launch(const Params& p, cudaStream_t st, const char* who) {
   const long long grid = run_blocks(p) * ((p.D / VEC + 31) / 32);
   TTT_REQUIRE(grid < (1LL << 31), TTT_ERR_SHAPE, "%s: %lld blocks are too many", who, grid);
-  if (BWD) conv_bwd_kernel<T, K, VEC><<<(unsigned)grid, kWarps * 32, 0, st>>>(p);
-  else conv_fwd_kernel<T, K, VEC><<<(unsigned)grid, kWarps * 32, 0, st>>>(p);
+  const auto kernel = [&] {
+    if constexpr (BWD) return p.seq ? conv_bwd_kernel<T, K, VEC, true> : conv_bwd_kernel<T, K, VEC, false>;
+    else return p.seq ? conv_fwd_kernel<T, K, VEC, true> : conv_fwd_kernel<T, K, VEC, false>;
+  }();
+  kernel<<<(unsigned)grid, kWarps * 32, 0, st>>>(p);
   return check_launch(who);
 }
 template <typename T, int VEC, bool BWD>
@@ -355,10 +451,10 @@ extern "C" int ttt_causal_conv_fwd(int rows, int L, int D, int K, const void* x,
   conv::Params p{};
   p.rows = rows, p.L = L, p.D = D, p.act = act, p.x = x, p.x_b = strides[0], p.x_l = strides[1];
   p.w = w, p.b = b, p.seq = seq, p.init = init, p.fin = fin, p.y = y;
-  const int elem = dt == DT_F32 ? 4 : 2, vec = 16 / elem;
-  const bool on = conv::vectors(D, vec, elem, strides, {x, init, fin, y});
-  conv::split(p, on ? vec : 1);
-  return conv::launch_t<8, 4, false>(p, K, dt, on, static_cast<cudaStream_t>(stream), who);
+  const int elem = dt == DT_F32 ? 4 : 2;
+  const bool on = conv::vectors(D, 4, elem, strides, {x, init, fin, y});
+  conv::split(p, on ? 4 : 1);
+  return conv::launch_t<4, 4, false>(p, K, dt, on, static_cast<cudaStream_t>(stream), who);
 }
 
 // The backward holds K rows of x, of gradients and of weight sums per channel: 8-byte vectors.

@@ -155,7 +155,7 @@ __device__ __forceinline__ void run_tile(const Params& p, const Where& w, const 
 // The first half of the CTA runs tile i while the second finishes the outputs of tile i - 1 and
 // prepares tile i + 1 in the other buffer; one barrier a tile.
 template <typename T, int LN, int NPT, bool SEQ>
-__global__ void __launch_bounds__(256, NPT == 4 ? 3 : 1) scan_fwd_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(256, NPT == 4 ? 3 : NPT == 8 ? 2 : 1) scan_fwd_kernel(const __grid_constant__ Params p) {
   using F = Fwd<LN, NPT>;
   extern __shared__ __align__(16) unsigned char raw_smem[];
   auto& s = *reinterpret_cast<typename F::Smem*>(raw_smem);
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 3 : 1) scan_fwd_kernel(const _
 // A piece's end state from zero (REV: the carry that leaves its first token from zero at its
 // last), and the sum of its step sizes.
 template <typename T, int LN, int NPT, bool REV, bool SEQ>
-__global__ void __launch_bounds__(256, NPT == 4 ? 3 : 1) scan_chunk_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(256, NPT == 4 ? 3 : NPT == 8 ? 2 : 1) scan_chunk_kernel(const __grid_constant__ Params p) {
   using F = Fwd<LN, NPT>;
   extern __shared__ __align__(16) unsigned char raw_smem[];
   auto& s = *reinterpret_cast<typename F::Smem*>(raw_smem);
@@ -531,8 +531,9 @@ int check_sizes(const char* who, int rows, int L, int D, int G, int N, int dt) {
 static int split(int rows, int L, int D, int G, int N, bool backward) {
   const int DT = 256 / shape_of(N).LN;
   const long long blocks = (long long)rows * G * ((D / G + DT - 1) / DT);
-  const bool narrow = shape_of(N).NPT == 4;
-  return backward ? piece_tokens(blocks, L, narrow ? 2 : 1, 0.3f) : piece_tokens(blocks, L, narrow ? 3 : 1, 0.5f);
+  const int NPT = shape_of(N).NPT;  // resident CTAs as the kernels' launch bounds have them
+  return backward ? piece_tokens(blocks, L, NPT == 4 ? 2 : 1, 0.3f)
+                  : piece_tokens(blocks, L, NPT == 4 ? 3 : NPT == 8 ? 2 : 1, 0.5f);
 }
 void plan_pieces(Params& p, bool backward) {
   p.chunk = split(p.rows, p.L, p.D, p.G, p.N, backward);
