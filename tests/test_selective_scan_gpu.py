@@ -311,3 +311,93 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for w, gs in zip(want, got):
         assert all(torch.equal(a, b) for g in gs for a, b in zip(w, g))
+
+
+def test_refusals():
+    t = {k: v.to(DEV) for k, v in make(2, 6, 8, 4, 1, torch.bfloat16, 1).items()}
+    good = lambda **kw: {**t, **kw}  # noqa: E731
+    for bad in (good(delta=t["delta"][:, :5]), good(A=t["A"][:4]), good(B=t["B"][..., :3]), good(C=t["C"].float()),
+                good(D=t["D"][:3]), good(z=t["z"][:1]), good(bias=t["bias"][:2]), good(init=torch.zeros(3, 8, 4, device=DEV)),
+                good(B=t["B"].expand(2, 6, 3, 4))):
+        with pytest.raises(ValueError):
+            call(bad)
+    with pytest.raises(ValueError, match="at most 128"):
+        call(good(A=torch.zeros(8, 129, device=DEV), B=t["B"][..., :1].expand(2, 6, 1, 129),
+                  C=t["C"][..., :1].expand(2, 6, 1, 129)))
+    with pytest.raises(TypeError):
+        call({k: v.double() for k, v in t.items()})
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        call(good(A=t["A"].cpu()))
+    with pytest.raises(ValueError, match="one row"):
+        call(t, cu=torch.tensor([0, 6], device=DEV, dtype=torch.int32))
+    s = {k: v[:, 0] if v.dim() > 2 else v for k, v in t.items()}
+    step = lambda st, ix=None, **kw: ops.selective_scan_step(  # noqa: E731
+        st, kw.get("u", s["u"]), s["delta"], s["A"], s["B"], s["C"], s["D"], s["z"], s["bias"], True, ix)
+    state = torch.zeros(2, 8, 4, device=DEV)
+    for st, ix in ((state.bfloat16(), None), (state[:1], None), (state[..., :3], None), (state.transpose(1, 2), None),
+                   (state[:1].expand(2, 8, 4), None), (state, torch.zeros(3, device=DEV, dtype=torch.int32)),
+                   (state, torch.zeros(2, device=DEV, dtype=torch.int64))):
+        with pytest.raises(ValueError):
+            step(st, ix)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        step(state, u=s["u"].clone().requires_grad_(True))
+    assert float(state.abs().max()) == 0
+
+
+def test_bad_sequence_offsets_stay_in_bounds():
+    """Offsets out of order, negative or past the end give some result, and touch nothing else."""
+    t = {k: v.to(DEV) for k, v in make(1, 70, 12, 16, 1, torch.float32, 6, 4).items()}
+    for cu in ([0, 50, 20, 60, 70], [-5, 10, 10, 200, 300], [70, 60, 30, 10, 0], [5, 9, 12, 40, 41]):
+        cud = torch.tensor(cu, device=DEV, dtype=torch.int32)
+        leaves = {k: v.clone().requires_grad_(True) for k, v in t.items()}
+        y, fin = call(leaves, cu=cud)
+        torch.autograd.grad([y, fin], list(leaves.values()), [torch.ones_like(y), torch.ones_like(fin)])
+        ops.causal_conv1d(t["u"], torch.ones(12, 4, device=DEV), cu_seqlens=cud)
+    torch.cuda.synchronize()
+
+
+def test_a_nan_stays_in_its_sequence():
+    """A NaN in one packed sequence reaches no output or gradient of the others' tokens."""
+    t = make(1, 60, 20, 16, 1, torch.bfloat16, 12, 4)
+    t["u"][0, 23, 3] = float("nan")
+    leaves = {k: v.to(DEV).requires_grad_(True) for k, v in t.items()}
+    cu = torch.tensor([0, 21, 26, 41, 60], device=DEV, dtype=torch.int32)
+    y, fin = call(leaves, cu=cu)
+    g = torch.autograd.grad([y, fin], [leaves[k] for k in ("u", "delta", "B", "C", "z", "init")],
+                            [torch.ones_like(y), torch.ones_like(fin)])
+    keep = torch.cat([torch.arange(21), torch.arange(26, 60)]).to(DEV)
+    for v in (y, *g[:5]):
+        assert bool(torch.isfinite(v[:, keep]).all())
+    assert bool(torch.isfinite(fin[[0, 2, 3]]).all()) and bool(torch.isfinite(g[5][[0, 2, 3]]).all())
+    assert bool(fin[1].isnan().any())
+
+
+def test_another_stream_than_the_tensors_own():
+    t = {k: v.to(DEV) for k, v in make(2, 300, 24, 16, 1, torch.float32, 17, 2).items()}
+    want = call(t)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = call(t)
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_parameters_in_16_bits_and_shared_leaves():
+    """A, D and the bias in bf16 get bf16 gradients; one tensor as both B and C, and an expanded
+    u, add their gradients."""
+    t = {k: v.to(DEV) for k, v in make(2, 40, 16, 16, 1, torch.float32, 19).items()}
+    for k in ("A", "D", "bias"):
+        t[k] = t[k].bfloat16()
+    u = t["u"][:1].clone().requires_grad_(True)
+    bc = t["B"].clone().requires_grad_(True)
+    A = t["A"].requires_grad_(True)
+    y = call({**t, "u": u.expand(2, 40, 16), "B": bc, "C": bc, "A": A}, final=False)
+    dy = torch.randn_like(y)
+    got = torch.autograd.grad(y, [u, bc, A], dy)
+    ud, bd, Ad = (x.detach().double().cpu().requires_grad_(True) for x in (u, bc, A))
+    c = {k: v.detach().double().cpu() for k, v in t.items()}
+    ry, _ = R.selective_scan(ud.expand(2, 40, 16), c["delta"], Ad, bd, bd, c["D"], c["z"], c["bias"], True)
+    want = torch.autograd.grad(ry, [ud, bd, Ad], dy.double().cpu())
+    for a, b in zip(got, want):
+        assert R.rel(a, b) <= tol(a.dtype, 40, 16, 16)

@@ -3,7 +3,7 @@
     python ttt-triton_b200/build.py [--force] [--phase-stamps]
 
 The library is a plain C-ABI shared object (include/ttt_b200.h); nothing here links
-against torch. The build is incremental on source modification times. ``--phase-stamps``
+against torch. The sources are compiled side by side, one nvcc each. The build is incremental on source modification times. ``--phase-stamps``
 builds a second library, libttt_b200_stamps.so, whose TTT-MLP tensor-core forward records a
 per-phase %globaltimer timeline (phase_timeline.py reads it); the product library has none.
 """
@@ -15,6 +15,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
@@ -23,7 +25,7 @@ LIB = os.path.join(HERE, "libttt_b200.so")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
     "--expt-relaxed-constexpr",
 ]
 
@@ -58,12 +60,20 @@ def build(force=False, verbose=False, phase_stamps=False):
         return lib
     tmp = lib + ".tmp"
     extra = ["-DTTT_PHASE_STAMPS"] if phase_stamps else []
-    cmd = [_nvcc(), *NVCC_FLAGS, *extra, "-I", os.path.join(REPO, "include"), "-o", tmp, *sources()]
-    if verbose:
-        print(" ".join(cmd))
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+
+    def run(cmd):
+        if verbose:
+            print(" ".join(cmd))
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+
+    with tempfile.TemporaryDirectory() as work:
+        objects = {src: os.path.join(work, os.path.basename(src) + ".o") for src in sources()}
+        with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+            list(pool.map(lambda src: run([_nvcc(), *NVCC_FLAGS, *extra, "-I", os.path.join(REPO, "include"), "-c",
+                                           "-o", objects[src], src]), objects))
+        run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", tmp, *objects.values()])
     os.replace(tmp, lib)
     return lib
 

@@ -15,6 +15,11 @@ Parameter names match the reference's modules, so its state dicts load
 16-bit training the reference gets from autocast); parameters and the inner states stay
 fp32.
 
+``SelectiveScanLayer`` is the other kind of layer the forecaster can stack
+(``ssm_layer="selective_scan"``; the reference's name for the choice of scan): input
+projection, causal convolution, selective scan, gate and output projection on
+``ops.causal_conv1d`` and ``ops.selective_scan``, with a single-token form for serving.
+
 ``train_step`` is one optimisation step of main.py:73-100 (AdamW, MSE, gradient clipping at
 1.0); under torch.distributed the model is wrapped in DistributedDataParallel and the
 outer-parameter gradients are averaged by NCCL all-reduce over NVLink.
@@ -22,11 +27,14 @@ outer-parameter gradients are averaged by NCCL all-reduce over NVLink.
 
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn.functional as Fn
 from torch import nn
 
 import epilogue
+import ops
 import prologue
 from kernels.mlp_memo_mix import mlp_memo_mix
 from mlp_triton import TritonMLP
@@ -152,18 +160,82 @@ def linear_act(x, weight, bias, dt):
     return Fn.linear(x.to(dt), torch.cat(cols, 1).to(dt))
 
 
+class SelectiveScanLayer(nn.Module):
+    """A sequence layer on the selective scan: x, z = in_proj(hidden); x through the causal
+    convolution and a silu; step sizes (a low-rank projection), B and C from x; the scan gated
+    by z; out_proj. Parameters fp32, activations in act_dtype, states fp32."""
+
+    def __init__(self, model_dim, state_size=16, expand=2, conv_taps=4, dt_rank=None, act_dtype=torch.bfloat16):
+        super().__init__()
+        W = model_dim * expand
+        R = dt_rank if dt_rank is not None else -(-model_dim // 16)
+        self.inner, self.state_size, self.dt_rank, self.act_dtype = W, state_size, R, act_dtype
+        self.in_proj = nn.Linear(model_dim, 2 * W, bias=False)
+        self.conv_weight = nn.Parameter(torch.empty(W, conv_taps).uniform_(-1, 1) / conv_taps**0.5)
+        self.conv_bias = nn.Parameter(torch.zeros(W))
+        self.x_proj = nn.Linear(W, R + 2 * state_size, bias=False)
+        self.dt_proj = nn.Linear(R, W)
+        # step sizes of 0.001 to 0.1 through the softplus, decays of -1 .. -N
+        dt = torch.exp(torch.empty(W).uniform_(math.log(1e-3), math.log(1e-1)))
+        with torch.no_grad():
+            self.dt_proj.bias.copy_(dt + torch.log(-torch.expm1(-dt)))
+        self.A_log = nn.Parameter(torch.log(torch.arange(1, state_size + 1).float()).repeat(W, 1))
+        self.D = nn.Parameter(torch.ones(W))
+        self.out_proj = nn.Linear(W, model_dim, bias=False)
+
+    def _scan_inputs(self, x):
+        """Step sizes before their bias, B and C of the convolved x [.., W]."""
+        dt = self.act_dtype
+        d, B, C = Fn.linear(x, self.x_proj.weight.to(dt)).split([self.dt_rank, self.state_size, self.state_size], -1)
+        return Fn.linear(d, self.dt_proj.weight.to(dt)), B, C
+
+    def forward(self, hidden_states, state=None, cu_seqlens=None, return_state=False):
+        """hidden_states [B, L, model_dim], or [1, T, model_dim] packed by cu_seqlens; state and
+        the one returned with return_state: (convolution rows, scan state) per sequence."""
+        dt = self.act_dtype
+        x, z = Fn.linear(hidden_states.to(dt), self.in_proj.weight.to(dt)).chunk(2, -1)
+        conv0, scan0 = state if state is not None else (None, None)
+        x, conv1 = ops.causal_conv1d(x, self.conv_weight, self.conv_bias, "silu", conv0, cu_seqlens, True)
+        delta, B, C = self._scan_inputs(x)
+        y, scan1 = ops.selective_scan(x, delta, -torch.exp(self.A_log), B, C, self.D, z, self.dt_proj.bias, True, scan0,
+                                      cu_seqlens, True)
+        out = Fn.linear(y, self.out_proj.weight.to(dt))
+        return (out, (conv1, scan1)) if return_state else out
+
+    def new_state(self, slots, device=None):
+        """Zero state of `slots` sequences for ``step``."""
+        dev = device if device is not None else self.D.device
+        return (torch.zeros(slots, self.conv_weight.shape[1] - 1, self.inner, device=dev, dtype=self.act_dtype),
+                torch.zeros(slots, self.inner, self.state_size, device=dev, dtype=torch.float32))
+
+    @torch.no_grad()
+    def step(self, hidden_states, state, state_indices=None):
+        """One new token per sequence, hidden_states [B, model_dim]; state is updated in place."""
+        dt = self.act_dtype
+        x, z = Fn.linear(hidden_states.to(dt), self.in_proj.weight.to(dt)).chunk(2, -1)
+        x = ops.causal_conv1d_step(x, state[0], self.conv_weight, self.conv_bias, "silu", state_indices)
+        delta, B, C = self._scan_inputs(x)
+        y = ops.selective_scan_step(state[1], x, delta, -torch.exp(self.A_log), B, C, self.D, z, self.dt_proj.bias, True,
+                                    state_indices)
+        return Fn.linear(y, self.out_proj.weight.to(dt))
+
+
 class TTTForecaster(nn.Module):
     """forecast.TTTForecaster (in_proj -> TTT layers -> head on the last position) with
-    num_layers stacked TTT-MLP layers."""
+    num_layers stacked TTT-MLP layers, or selective scan layers with ssm_layer="selective_scan"
+    (num_heads and the ttt_ and scan_ settings are the TTT-MLP's)."""
 
     def __init__(self, d_in, d_out, pred_len, seq_len, model_dim=256, num_heads=4, num_layers=4,
                  mini_batch_size=16, ttt_base_lr=0.1, scan_checkpoint_group_size=16,
-                 mem_cache_segment_n_mini_batches=2, act_dtype=torch.bfloat16):
+                 mem_cache_segment_n_mini_batches=2, act_dtype=torch.bfloat16, ssm_layer="ttt_mlp"):
         super().__init__()
+        if ssm_layer not in ("ttt_mlp", "selective_scan"):
+            raise ValueError(f"ssm_layer must be 'ttt_mlp' or 'selective_scan', got {ssm_layer!r}")
         self.pred_len, self.d_out = pred_len, d_out
         self.act_dtype = act_dtype
         self.in_proj = nn.Linear(d_in, model_dim)
         self.layers = nn.ModuleList(
+            SelectiveScanLayer(model_dim, act_dtype=act_dtype) if ssm_layer == "selective_scan" else
             TTTMLPLayer(model_dim, num_heads, mini_batch_size, seq_len, ttt_base_lr, scan_checkpoint_group_size,
                         mem_cache_segment_n_mini_batches, act_dtype=act_dtype) for _ in range(num_layers))
         self.head = nn.Linear(model_dim, pred_len * d_out)
@@ -254,5 +326,5 @@ def tokens_per_step(batch, seq_len, num_heads, num_layers):
     return batch * num_heads * seq_len * num_layers
 
 
-__all__ = ["BatchCopies", "linear_act", "TTTMLPLayer", "TTTForecaster", "rope_table_3d", "load_reference_state_dict", "make_optimizer",
+__all__ = ["BatchCopies", "linear_act", "TTTMLPLayer", "SelectiveScanLayer", "TTTForecaster", "rope_table_3d", "load_reference_state_dict", "make_optimizer",
            "train_step", "GraphedTrainStep", "tokens_per_step"]
