@@ -165,52 +165,64 @@ def selective_scan_backward(u, delta, A, B, C, D, z, delta_bias, softplus, init,
 
 def _check_step(state, index, rows, inputs, shape):
     """The carried state and the slots of a single-token call."""
-    if state.dim() != 3 or tuple(state.shape[1:]) != shape:
-        raise ValueError(f"the state must be [slots, {shape[0]}, {shape[1]}], got {tuple(state.shape)}")
-    if state.stride(2) != 1 or state.stride(1) != shape[1]:
+    size, stride = state.shape, state.stride()
+    if len(size) != 3 or size[1:] != shape:
+        raise ValueError(f"the state must be [slots, {shape[0]}, {shape[1]}], got {tuple(size)}")
+    if stride[2] != 1 or stride[1] != shape[1]:
         raise ValueError("the state is updated in place: each slot must be contiguous")
-    if state.shape[0] > 1 and state.stride(0) < shape[0] * shape[1]:
+    if size[0] > 1 and stride[0] < shape[0] * shape[1]:
         raise ValueError("the state's slots must not overlap")
     if index is None:
-        if state.shape[0] != rows:
+        if size[0] != rows:
             raise ValueError(f"{rows} rows need a state of {rows} slots or state_indices, got {state.shape[0]} slots")
     elif index.dim() != 1 or index.numel() != rows or index.dtype != torch.int32 or not index.is_contiguous():
         raise ValueError(f"state_indices must be contiguous int32 [{rows}]")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in inputs if t is not None):
+    if torch.is_grad_enabled() and any([t.requires_grad for t in inputs if t is not None]):
         raise RuntimeError("the single-token step has no gradient: call it under torch.no_grad()")
+
+
+def _check_devices(tensors):
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev or dev < 0:
+            require_cuda(*(t for t in tensors if t is not None))
 
 
 @_on_tensor_device
 def selective_scan_step(state, u, delta, A, B, C, D, z, delta_bias, softplus, index):
     """One token per row: out [B, D]; state [slots, D, N] fp32 updated in place."""
-    inputs = (state, u, delta, A, B, C, D, z, delta_bias)
-    require_cuda(*[t for t in (*inputs, index) if t is not None])
-    if u.dim() != 2:
-        raise ValueError(f"u must be [B, D], got shape {tuple(u.shape)}")
-    rows, W = u.shape
+    _check_devices((u, state, delta, A, B, C, D, z, delta_bias, index))
+    shape = u.shape
+    if len(shape) != 2:
+        raise ValueError(f"u must be [B, D], got shape {tuple(shape)}")
+    rows, W = shape
     if A.dim() != 2 or A.shape[0] != W or not 1 <= A.shape[1] <= MAX_STATES:
         raise ValueError(f"A must be [{W}, N] with N from 1 to {MAX_STATES}, got {tuple(A.shape)}")
     N = A.shape[1]
-    _shaped("delta", delta, u.shape)
-    _shaped("z", z, u.shape)
-    if B.dim() != 3 or B.shape[0] != rows or B.shape[2] != N or B.shape[1] < 1 or W % B.shape[1]:
-        raise ValueError(f"B must be [{rows}, {N}] or [{rows}, G, {N}] with G dividing {W}, got {tuple(B.shape)}")
-    _shaped("C", C, B.shape)
+    bs = B.shape
+    if len(bs) != 3 or bs[0] != rows or bs[2] != N or bs[1] < 1 or W % bs[1]:
+        raise ValueError(f"B must be [{rows}, {N}] or [{rows}, G, {N}] with G dividing {W}, got {tuple(bs)}")
+    _shaped("delta", delta, shape)
+    _shaped("z", z, shape)
+    _shaped("C", C, bs)
     _shaped("D", D, (W,))
     _shaped("delta_bias", delta_bias, (W,))
-    _same(u, delta=delta, B=B, C=C, z=z)
+    dt = u.dtype
+    if delta.dtype != dt or B.dtype != dt or C.dtype != dt or (z is not None and z.dtype != dt):
+        _same(u, delta=delta, B=B, C=C, z=z)
     if state.dtype != torch.float32:
         raise ValueError(f"the state must be float32, got {state.dtype}")
-    _check_step(state, index, rows, inputs, (W, N))
-    out = torch.empty(rows, W, device=u.device, dtype=u.dtype)
-    if rows == 0:
-        return out
+    _check_step(state, index, rows, (state, u, delta, A, B, C, D, z, delta_bias), (W, N))
     u, delta, B, C = _rows(u), _rows(delta), _rows(B), _rows(C)
     z = _rows(z) if z is not None else None
+    out = torch.empty(shape, device=u.device, dtype=dt)
+    if rows == 0:
+        return out
     A, D, delta_bias = _f32(A), _f32(D), _f32(delta_bias)
-    st = _strides(u.stride(0), delta.stride(0), B.stride(0), B.stride(1), C.stride(0), C.stride(1),
-                  z.stride(0) if z is not None else 0, state.stride(0))
-    check(lib.ttt_selective_scan_step(rows, W, B.shape[1], N, state.shape[0], ptr(u), ptr(delta), ptr(B), ptr(C), ptr(z),
+    bt, ct = B.stride(), C.stride()
+    st = _strides(u.stride(0), delta.stride(0), bt[0], bt[1], ct[0], ct[1], z.stride(0) if z is not None else 0,
+                  state.stride(0))
+    check(lib.ttt_selective_scan_step(rows, W, bs[1], N, state.shape[0], ptr(u), ptr(delta), ptr(B), ptr(C), ptr(z),
                                       dtype_code(u), st, ptr(A), ptr(D), ptr(delta_bias), int(softplus), ptr(index),
                                       ptr(state), ptr(out), stream_of(u)), "ttt_selective_scan_step")
     return out
@@ -285,7 +297,7 @@ def causal_conv_backward(x, w, b, act, init, seq, dy, dfin, want_dinit):
 @_on_tensor_device
 def causal_conv_step(x, state, weight, bias, activation, index):
     """One token per row: y [B, D]; state [slots, K - 1, D] shifted in place."""
-    require_cuda(*(t for t in (x, state, weight, bias, index) if t is not None))
+    _check_devices((x, state, weight, bias, index))
     act = _act_code(activation)
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"x must be [B, D], got shape {tuple(x.shape)}")

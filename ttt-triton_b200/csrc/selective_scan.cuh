@@ -309,8 +309,9 @@ __device__ __forceinline__ float2 state_sums(const float* y) {
 // that is kept for a thousand tokens multiplies. Half a step of 2^-24 on the argument brings
 // the average to 0.05 * 2^-24 and costs nothing (a fused multiply-add for a product); a step
 // size of zero still gives exactly 1.
+constexpr float kHalfStep = 2.9802322387695312e-8f;  // 2^-25
 __device__ __forceinline__ float2 decay(float2 dt, float2 A2) {
-  const float2 x = __ffma2_rn(dt, A2, all2(2.9802322387695312e-8f));
+  const float2 x = __ffma2_rn(dt, A2, all2(kHalfStep));
   return make_float2(ex2(x.x), ex2(x.y));
 }
 

@@ -20,6 +20,7 @@
 #pragma once
 
 #include "selective_scan.cuh"
+
 namespace ttt {
 namespace scan {
 
@@ -161,111 +162,111 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
       if (SEQ) mask = warp_masks<F::TB>(p.seq, tt, tend, p.L);
 #pragma unroll 1
       for (int t0 = tt + (F::RUNS - 1) * F::SUB; t0 >= tt; t0 -= F::SUB) {
-      if (t0 >= tend) continue;
-      const int b = t0 - tt;
-      const auto tokens = [&](auto checks) {
-        constexpr bool CHECK = decltype(checks)::value;
-        float2 a[F::SUB][2][H], ah[F::SUB][2][H];
-        asm volatile("cp.async.wait_group %0;" ::"n"(F::RING - 2) : "memory");
-        Both<NPT> h;
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int e = 0; e < NPT / 4; ++e) {
-            const float4 q = s.kept[run % F::RING][tid + (c * (NPT / 4) + e) * F::MAIN];
-            h.c[c].v[2 * e] = make_float2(q.x, q.y), h.c[c].v[2 * e + 1] = make_float2(q.z, q.w);
-          }
-        fetch_states(run - (F::RING - 1));
-        --run;
-#pragma unroll
-        for (int k = 0; k < F::SUB; ++k) {
-          if constexpr (CHECK && SEQ) {
-            if (mask.start >> (b + k) & 1) {
-              const int sq = p.seq[t0 + k];
-              h = load2(p.init + sq * DN, sq >= 0 && p.init);
-            }
-          }
-          const float4 d4 = *reinterpret_cast<const float4*>(&tile.d[(b + k) * F::DT + cl]);
-          const Pairs<NPT> B2 = row_pairs<NPT>(tile.B + (b + k) * F::NP + n0);
+        if (t0 >= tend) continue;
+        const int b = t0 - tt;
+        const auto tokens = [&](auto checks) {
+          constexpr bool CHECK = decltype(checks)::value;
+          float2 a[F::SUB][2][H], ah[F::SUB][2][H];
+          asm volatile("cp.async.wait_group %0;" ::"n"(F::RING - 2) : "memory");
+          Both<NPT> h;
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int j = 0; j < H; ++j) {
-              a[k][c][j] = decay(all2(c ? d4.z : d4.x), A2.c[c].v[j]);
-              ah[k][c][j] = __fmul2_rn(a[k][c][j], h.c[c].v[j]);
-              h.c[c].v[j] = __ffma2_rn(all2(c ? d4.w : d4.y), B2.v[j], ah[k][c][j]);
+            for (int e = 0; e < NPT / 4; ++e) {
+              const float4 q = s.kept[run % F::RING][tid + (c * (NPT / 4) + e) * F::MAIN];
+              h.c[c].v[2 * e] = make_float2(q.x, q.y), h.c[c].v[2 * e + 1] = make_float2(q.z, q.w);
             }
-        }
-        // tokens of two sequences never share a product: a NaN of one would reach the other's columns
-        constexpr int TS = CHECK ? 1 : F::TS;
+          fetch_states(run - (F::RING - 1));
+          --run;
 #pragma unroll
-        for (int g0 = F::SUB - TS; g0 >= 0; g0 -= TS) {
-          float accB[H][4], accC[H][4];
-#pragma unroll
-          for (int j = 0; j < H; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) accB[j][e] = accC[j][e] = 0.f;
-#pragma unroll
-          for (int k = g0 + TS - 1; k >= g0; --k) {
-            if constexpr (CHECK) {
-              if (t0 + k >= tend) continue;
-              if (SEQ && (mask.end >> (b + k) & 1)) {
+          for (int k = 0; k < F::SUB; ++k) {
+            if constexpr (CHECK && SEQ) {
+              if (mask.start >> (b + k) & 1) {
                 const int sq = p.seq[t0 + k];
-                carry = load2(p.dfin + sq * DN, sq >= 0 && p.dfin);
+                h = load2(p.init + sq * DN, sq >= 0 && p.init);
               }
             }
             const float4 d4 = *reinterpret_cast<const float4*>(&tile.d[(b + k) * F::DT + cl]);
-            const float2 dy2 = *reinterpret_cast<const float2*>(&tile.dy[(b + k) * F::DT + cl]);
-            const Pairs<NPT> B2 = row_pairs<NPT>(tile.B + (b + k) * F::NP + n0), C2 = row_pairs<NPT>(tile.C + (b + k) * F::NP + n0);
-            const float one = col_tok == k - g0 ? 1.f : 0.f;
-            const float2 zero = all2(0.f);
-            float2 s1[2] = {zero, zero}, s2[2] = {zero, zero}, s3[2] = {zero, zero};
+            const Pairs<NPT> B2 = row_pairs<NPT>(tile.B + (b + k) * F::NP + n0);
 #pragma unroll
-            for (int j = 0; j < H; ++j) {
-              float2 g[2], hn[2];
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const float2 ahj = ah[k][c][j];
-                g[c] = __ffma2_rn(C2.v[j], all2(c ? dy2.y : dy2.x), carry.c[c].v[j]);
-                hn[c] = __ffma2_rn(all2(c ? d4.w : d4.y), B2.v[j], ahj);
-                const float2 q = __fmul2_rn(g[c], ahj);
-                s1[c] = j ? __ffma2_rn(g[c], B2.v[j], s1[c]) : __fmul2_rn(g[c], B2.v[j]);
-                s2[c] = j ? __ffma2_rn(q, A2.c[c].v[j], s2[c]) : __fmul2_rn(q, A2.c[c].v[j]);
-                s3[c] = j ? __ffma2_rn(hn[c], C2.v[j], s3[c]) : __fmul2_rn(hn[c], C2.v[j]);
-                dA.c[c].v[j] = __ffma2_rn(q, all2(c ? d4.z : d4.x), dA.c[c].v[j]);
-                carry.c[c].v[j] = __fmul2_rn(a[k][c][j], g[c]);
-              }
-              add_over_channels<SPLIT>(accB[j], __ffma2_rn(g[0], all2(d4.y), __fmul2_rn(g[1], all2(d4.w))), one);
-              add_over_channels<SPLIT>(accC[j], __ffma2_rn(hn[0], all2(dy2.x), __fmul2_rn(hn[1], all2(dy2.y))), one);
-            }
-            const int o = ((b + k) * LN + nl) * F::YS + cl;
-            *reinterpret_cast<float2*>(&tile.s1[o]) = make_float2(s1[0].x + s1[0].y, s1[1].x + s1[1].y);
-            *reinterpret_cast<float2*>(&tile.s2[o]) = make_float2(s2[0].x + s2[0].y, s2[1].x + s2[1].y);
-            *reinterpret_cast<float2*>(&tile.s3[o]) = make_float2(s3[0].x + s3[0].y, s3[1].x + s3[1].y);
-            if constexpr (CHECK && SEQ) {
-              if (p.dinit && (mask.start >> (b + k) & 1)) {
-                const int sq = p.seq[t0 + k];
-                store_both<NPT>(p.dinit + sq * DN, d, n0, p.N, sq >= 0 && c0, sq >= 0 && c1, carry);
-              }
-            }
-          }
-          // of the products' two columns in this lane, those of the row's own channel group
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int c = 2 * l3 + e, tc = c / F::CG;
-            if (c % F::CG == cg && tc < TS) {
-              const int o = (b + g0 + tc) * F::NP + n0;
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
               for (int j = 0; j < H; ++j) {
-                *reinterpret_cast<float2*>(&tile.dB[warp * F::CG + cg][o + 2 * j]) = make_float2(accB[j][e], accB[j][2 + e]);
-                *reinterpret_cast<float2*>(&tile.dC[warp * F::CG + cg][o + 2 * j]) = make_float2(accC[j][e], accC[j][2 + e]);
+                a[k][c][j] = decay(all2(c ? d4.z : d4.x), A2.c[c].v[j]);
+                ah[k][c][j] = __fmul2_rn(a[k][c][j], h.c[c].v[j]);
+                h.c[c].v[j] = __ffma2_rn(all2(c ? d4.w : d4.y), B2.v[j], ah[k][c][j]);
+              }
+          }
+          // tokens of two sequences never share a product: a NaN of one would reach the other's columns
+          constexpr int TS = CHECK ? 1 : F::TS;
+#pragma unroll
+          for (int g0 = F::SUB - TS; g0 >= 0; g0 -= TS) {
+            float accB[H][4], accC[H][4];
+#pragma unroll
+            for (int j = 0; j < H; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) accB[j][e] = accC[j][e] = 0.f;
+#pragma unroll
+            for (int k = g0 + TS - 1; k >= g0; --k) {
+              if constexpr (CHECK) {
+                if (t0 + k >= tend) continue;
+                if (SEQ && (mask.end >> (b + k) & 1)) {
+                  const int sq = p.seq[t0 + k];
+                  carry = load2(p.dfin + sq * DN, sq >= 0 && p.dfin);
+                }
+              }
+              const float4 d4 = *reinterpret_cast<const float4*>(&tile.d[(b + k) * F::DT + cl]);
+              const float2 dy2 = *reinterpret_cast<const float2*>(&tile.dy[(b + k) * F::DT + cl]);
+              const Pairs<NPT> B2 = row_pairs<NPT>(tile.B + (b + k) * F::NP + n0), C2 = row_pairs<NPT>(tile.C + (b + k) * F::NP + n0);
+              const float one = col_tok == k - g0 ? 1.f : 0.f;
+              const float2 zero = all2(0.f);
+              float2 s1[2] = {zero, zero}, s2[2] = {zero, zero}, s3[2] = {zero, zero};
+#pragma unroll
+              for (int j = 0; j < H; ++j) {
+                float2 g[2], hn[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                  const float2 ahj = ah[k][c][j];
+                  g[c] = __ffma2_rn(C2.v[j], all2(c ? dy2.y : dy2.x), carry.c[c].v[j]);
+                  hn[c] = __ffma2_rn(all2(c ? d4.w : d4.y), B2.v[j], ahj);
+                  const float2 q = __fmul2_rn(g[c], ahj);
+                  s1[c] = j ? __ffma2_rn(g[c], B2.v[j], s1[c]) : __fmul2_rn(g[c], B2.v[j]);
+                  s2[c] = j ? __ffma2_rn(q, A2.c[c].v[j], s2[c]) : __fmul2_rn(q, A2.c[c].v[j]);
+                  s3[c] = j ? __ffma2_rn(hn[c], C2.v[j], s3[c]) : __fmul2_rn(hn[c], C2.v[j]);
+                  dA.c[c].v[j] = __ffma2_rn(q, all2(c ? d4.z : d4.x), dA.c[c].v[j]);
+                  carry.c[c].v[j] = __fmul2_rn(a[k][c][j], g[c]);
+                }
+                add_over_channels<SPLIT>(accB[j], __ffma2_rn(g[0], all2(d4.y), __fmul2_rn(g[1], all2(d4.w))), one);
+                add_over_channels<SPLIT>(accC[j], __ffma2_rn(hn[0], all2(dy2.x), __fmul2_rn(hn[1], all2(dy2.y))), one);
+              }
+              const int o = ((b + k) * LN + nl) * F::YS + cl;
+              *reinterpret_cast<float2*>(&tile.s1[o]) = make_float2(s1[0].x + s1[0].y, s1[1].x + s1[1].y);
+              *reinterpret_cast<float2*>(&tile.s2[o]) = make_float2(s2[0].x + s2[0].y, s2[1].x + s2[1].y);
+              *reinterpret_cast<float2*>(&tile.s3[o]) = make_float2(s3[0].x + s3[0].y, s3[1].x + s3[1].y);
+              if constexpr (CHECK && SEQ) {
+                if (p.dinit && (mask.start >> (b + k) & 1)) {
+                  const int sq = p.seq[t0 + k];
+                  store_both<NPT>(p.dinit + sq * DN, d, n0, p.N, sq >= 0 && c0, sq >= 0 && c1, carry);
+                }
+              }
+            }
+            // of the products' two columns in this lane, those of the row's own channel group
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int c = 2 * l3 + e, tc = c / F::CG;
+              if (c % F::CG == cg && tc < TS) {
+                const int o = (b + g0 + tc) * F::NP + n0;
+#pragma unroll
+                for (int j = 0; j < H; ++j) {
+                  *reinterpret_cast<float2*>(&tile.dB[warp * F::CG + cg][o + 2 * j]) = make_float2(accB[j][e], accB[j][2 + e]);
+                  *reinterpret_cast<float2*>(&tile.dC[warp * F::CG + cg][o + 2 * j]) = make_float2(accC[j][e], accC[j][2 + e]);
+                }
               }
             }
           }
-        }
-      };
-      if (t0 + F::SUB > tend || (SEQ && ((mask.start | mask.end) >> b & ((1u << F::SUB) - 1)))) tokens(std::true_type{});
-      else tokens(std::false_type{});
+        };
+        if (t0 + F::SUB > tend || (SEQ && ((mask.start | mask.end) >> b & ((1u << F::SUB) - 1)))) tokens(std::true_type{});
+        else tokens(std::false_type{});
       }
       if (i % 8 == 7 || i + 1 == ntiles) {  // short sums first: a long chain of additions loses bits
 #pragma unroll

@@ -365,47 +365,61 @@ struct StepParams {
   void* out;         // [rows, D]
 };
 
-template <typename T, int LN, int NPT>
+// A CTA has 128 / LN channels of ROWS rows, whose states are all on their way before the first is
+// worked on: the state is read and written once, 8 N bytes a channel, and memory bounds it.
+template <typename T, int LN, int NPT, int ROWS>
 __global__ void __launch_bounds__(128) scan_step_kernel(const __grid_constant__ StepParams p) {
-  constexpr int DT = 128 / LN;
+  constexpr int DT = 128 / LN, H = NPT / 2;
   const int tid = threadIdx.x, nl = tid % LN, n0 = nl * NPT;
   const int tiles = (p.D + DT - 1) / DT;
-  const int row = blockIdx.x / tiles, d = (blockIdx.x - row * tiles) * DT + tid / LN;
+  const int row0 = (int)(blockIdx.x / tiles) * ROWS, d = (int)(blockIdx.x % tiles) * DT + tid / LN;
   const bool on = d < p.D;
-  const int ok = slot_state(p.index, row, p.slots);
-  if (ok <= 0) {
-    if (on && nl == 0)
-      static_cast<T*>(p.out)[(long long)row * p.D + d] = from_f<T>(ok < 0 ? __int_as_float(0x7fffffff) : 0.f);
-    return;
-  }
-  float y = 0.f, u = 0.f, z = 0.f;
-  if (on) {
-    float* state = p.state + (long long)(p.index ? p.index[row] : row) * p.state_b;
-    const int g = d / p.Dg;
-    u = to_f(static_cast<const T*>(p.u)[row * p.u_b + d]);
-    if (p.z) z = to_f(static_cast<const T*>(p.z)[row * p.z_b + d]);
-    const float dt = p.softplus
-                         ? softplus(to_f(static_cast<const T*>(p.delta)[row * p.delta_b + d]) + (p.bias ? p.bias[d] : 0.f))
-                         : to_f(static_cast<const T*>(p.delta)[row * p.delta_b + d]) + (p.bias ? p.bias[d] : 0.f);
-    const T* B = static_cast<const T*>(p.B) + row * p.B_b + g * p.B_g;
-    const T* C = static_cast<const T*>(p.C) + row * p.C_b + g * p.C_g;
+  int ok[ROWS];
+  float h[ROWS][NPT], A2[NPT];
+  float* state[ROWS];
 #pragma unroll
-    for (int i = 0; i < NPT; ++i) {
-      const int n = n0 + i;
-      if (n < p.N) {
-        const long long e = (long long)d * p.N + n;
-        const float h = fmaf(ex2(dt * (p.A[e] * kLog2e)), state[e], dt * u * to_f(B[n]));
-        state[e] = h;
-        y = fmaf(h, to_f(C[n]), y);
-      }
+  for (int r = 0; r < ROWS; ++r) {
+    const int row = row0 + r;
+    ok[r] = row < p.rows ? slot_state(p.index, row, p.slots) : 0;
+    state[r] = p.state + (ok[r] > 0 ? (p.index ? p.index[row] : row) * p.state_b : 0);
+    load_states<NPT>(state[r], d, n0, p.N, on && ok[r] > 0, h[r]);
+  }
+  load_states<NPT>(p.A, d, n0, p.N, on, A2);
+  const float skip = on && p.Dskip ? p.Dskip[d] : 0.f, bias = on && p.bias ? p.bias[d] : 0.f;
+  const int g = on ? d / p.Dg : 0;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int row = row0 + r;
+    if (row >= p.rows) break;
+    T* out = static_cast<T*>(p.out) + (long long)row * p.D + d;
+    if (ok[r] <= 0) {
+      if (on && nl == 0) *out = from_f<T>(ok[r] < 0 ? __int_as_float(0x7fffffff) : 0.f);
+      continue;
     }
-  }
+    float y = 0.f, u = 0.f, z = 0.f;
+    if (on) {
+      u = to_f(static_cast<const T*>(p.u)[row * p.u_b + d]);
+      if (p.z) z = to_f(static_cast<const T*>(p.z)[row * p.z_b + d]);
+      float dt = to_f(static_cast<const T*>(p.delta)[row * p.delta_b + d]) + bias;
+      if (p.softplus) dt = softplus(dt);
+      const T* B = static_cast<const T*>(p.B) + row * p.B_b + g * p.B_g + n0;
+      const T* C = static_cast<const T*>(p.C) + row * p.C_b + g * p.C_g + n0;
 #pragma unroll
-  for (int o = 1; o < LN; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-  if (on && nl == 0) {
-    if (p.Dskip) y = fmaf(p.Dskip[d], u, y);
-    if (p.z) y *= z * sigmoid(z);
-    static_cast<T*>(p.out)[(long long)row * p.D + d] = from_f<T>(y);
+      for (int i = 0; i < NPT; ++i) {
+        if (n0 + i < p.N) {
+          h[r][i] = fmaf(ex2(fmaf(dt, A2[i] * kLog2e, kHalfStep)), h[r][i], dt * u * to_f(B[i]));
+          y = fmaf(h[r][i], to_f(C[i]), y);
+        }
+      }
+      store_states<NPT>(state[r], d, n0, p.N, true, h[r]);
+    }
+#pragma unroll
+    for (int o = 1; o < LN; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+    if (on && nl == 0) {
+      y = fmaf(skip, u, y);
+      if (p.z) y *= z * sigmoid(z);
+      *out = from_f<T>(y);
+    }
   }
 }
 
@@ -496,8 +510,9 @@ bool couples(const Params& p, int dt) {
 // main pass's time, about 128 tokens' worth of launches and 3 a piece; it pays where the `blocks` CTAs of
 // whole rows leave SMs empty, or a last round of them nearly so. An SM runs `resident` CTAs at
 // once; k of them take 0.4 + 0.6 k / resident of that time. Measured, 16 x 2048 x 1536 states
-// of 16: backward 1.32 ms whole (384 CTAs on 296 places), EEE in 3 pieces; forward prompt of
-// 1 x 8192 x 1024: FFF whole, GGG in 26 pieces.
+// of 16: backward 1.32 ms whole (384 CTAs on 296 places), 1.44 ms in 3 pieces, whose first pass
+// alone takes 0.29 ms; 32 x 336 x 512 training 420 us in 4 pieces, 225 us whole; 1 x 8192 x 1024
+// prompt 160 us in 128 pieces, 123 us in 26.
 int piece_tokens(long long blocks, int L, int resident, float extra) {
   const long long sms = sm_count(), places = sms * resident;
   float best = 0.f;
@@ -620,11 +635,19 @@ extern "C" int ttt_selective_scan_step(int rows, int D, int G, int N, int slots,
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return scan::dispatch(N, [&](auto ln, auto npt) {
     constexpr int LN = decltype(ln)::value, NPT = decltype(npt)::value, DT = 128 / LN;
-    const long long grid = (long long)((D + DT - 1) / DT) * rows;
+    // four rows a CTA once one row each would be over 16 CTAs an SM: fewer, with more loads in flight
+    const long long tiles = (D + DT - 1) / DT;
+    const int each = tiles * rows > 16LL * scan::sm_count() ? 4 : 1;
+    const long long grid = tiles * ((rows + each - 1) / each);
     TTT_REQUIRE(grid < (1LL << 31), TTT_ERR_SHAPE, "%s: %lld blocks are too many", who, grid);
-    if (dt == DT_BF16) scan::scan_step_kernel<__nv_bfloat16, LN, NPT><<<(unsigned)grid, 128, 0, st>>>(p);
-    else if (dt == DT_F16) scan::scan_step_kernel<__half, LN, NPT><<<(unsigned)grid, 128, 0, st>>>(p);
-    else scan::scan_step_kernel<float, LN, NPT><<<(unsigned)grid, 128, 0, st>>>(p);
+    const auto go = [&](auto zero) {
+      using T = decltype(zero);
+      auto kernel = each == 4 ? scan::scan_step_kernel<T, LN, NPT, 4> : scan::scan_step_kernel<T, LN, NPT, 1>;
+      kernel<<<(unsigned)grid, 128, 0, st>>>(p);
+    };
+    if (dt == DT_BF16) go(__nv_bfloat16{});
+    else if (dt == DT_F16) go(__half{});
+    else go(float{});
     return check_launch(who);
   });
 }
