@@ -401,3 +401,27 @@ def test_parameters_in_16_bits_and_shared_leaves():
     want = torch.autograd.grad(ry, [ud, bd, Ad], dy.double().cpu())
     for a, b in zip(got, want):
         assert R.rel(a, b) <= tol(a.dtype, 40, 16, 16)
+
+
+def test_no_states_are_kept_without_a_gradient(monkeypatch):
+    """Under no_grad, parameters that require gradients or not, the forward keeps no states."""
+    import _scan_core as core
+
+    asked = []
+    real = core.selective_scan_forward
+    monkeypatch.setattr(core, "selective_scan_forward", lambda *a: asked.append(a[-1]) or real(*a))
+    t = {k: v.to(DEV) for k, v in make(1, 20, 8, 4, 1, torch.float32, 1).items()}
+    t["A"].requires_grad_(True)
+    with torch.no_grad():
+        y0, _ = call(t)
+    y1, _ = call(t)
+    assert asked == [False, True] and not y0.requires_grad and y1.requires_grad and torch.equal(y0, y1)
+
+
+def test_another_device_than_the_current_one():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one device")
+    t = {k: v.to("cuda:1") for k, v in make(1, 300, 8, 16, 1, torch.float32, 1, 1).items()}
+    y, fin = call(t)
+    ry, rfin = call({k: v.to("cuda:0") for k, v in t.items()})
+    assert torch.equal(y.cpu(), ry.cpu()) and torch.equal(fin.cpu(), rfin.cpu())

@@ -66,6 +66,12 @@ def sequence_index(cu_seqlens, T):
     return seq
 
 
+def training(*tensors):
+    """Whether a call has a gradient to prepare for. (Inside an autograd function's forward both
+    the mode and the inputs' flags say something else.)"""
+    return torch.is_grad_enabled() and any([t.requires_grad for t in tensors if t is not None])
+
+
 def packed(cu_seqlens, x):
     """(number of sequences, checked int32 offsets) of a batch of shape x.shape[:2]."""
     if cu_seqlens is None:

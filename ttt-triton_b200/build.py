@@ -3,8 +3,8 @@
     python ttt-triton_b200/build.py [--force] [--phase-stamps]
 
 The library is a plain C-ABI shared object (include/ttt_b200.h); nothing here links
-against torch. The sources are compiled side by side, one nvcc each. The build is incremental on source modification times. ``--phase-stamps``
-builds a second library, libttt_b200_stamps.so, whose TTT-MLP tensor-core forward records a
+against torch. The sources are compiled side by side, one nvcc each. The build is
+incremental on source modification times. ``--phase-stamps`` builds a second library, libttt_b200_stamps.so, whose TTT-MLP tensor-core forward records a
 per-phase %globaltimer timeline (phase_timeline.py reads it); the product library has none.
 """
 

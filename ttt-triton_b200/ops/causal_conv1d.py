@@ -29,9 +29,8 @@ class CausalConv1d(torch.autograd.Function):
         x, w, b = core._rows(x), core._f32(weight), core._f32(bias)
         init = init.contiguous() if init is not None else None
         y, fin = core.causal_conv_forward(x, w, b, act, init, seq, nseq, want_final)
-        if any(ctx.needs_input_grad):
-            ctx.act = act
-            ctx.save_for_backward(x, w, b, init, seq)
+        ctx.act = act
+        ctx.save_for_backward(x, w, b, init, seq)
         return y, fin
 
     @staticmethod
@@ -57,7 +56,12 @@ def causal_conv1d(x, weight, bias=None, activation=None, initial_state=None, cu_
     if cu is not None:
         core.require_cuda(x, cu)
         seq = core.sequence_index(cu, x.shape[1])
-    y, fin = CausalConv1d.apply(x, weight, bias, initial_state, act, seq, nseq, bool(return_final_state))
+    if core.training(x, weight, bias, initial_state):
+        y, fin = CausalConv1d.apply(x, weight, bias, initial_state, act, seq, nseq, bool(return_final_state))
+    else:
+        init = initial_state.contiguous() if initial_state is not None else None
+        y, fin = core.causal_conv_forward(core._rows(x), core._f32(weight), core._f32(bias), act, init, seq, nseq,
+                                          bool(return_final_state))
     return (y, fin) if return_final_state else y
 
 

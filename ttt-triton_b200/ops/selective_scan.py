@@ -26,21 +26,23 @@ from torch.autograd.function import once_differentiable
 import _scan_core as core
 
 
+def _layouts(u, delta, A, B, C, D, z, delta_bias):
+    """The inputs as the kernels read them."""
+    return (core._rows(u), core._rows(delta), core._f32(A), core._rows(B), core._rows(C), core._f32(D),
+            core._rows(z) if z is not None else None, core._f32(delta_bias))
+
+
 class SelectiveScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, u, delta, A, B, C, D, z, delta_bias, init, softplus, seq, nseq, want_final):
-        train = any(ctx.needs_input_grad)
         ctx.set_materialize_grads(False)
         ctx.param_dtypes = (A.dtype, D.dtype if D is not None else None,
                             delta_bias.dtype if delta_bias is not None else None,
                             init.dtype if init is not None else None)
-        args = (*(core._rows(t) for t in (u, delta)), core._f32(A), *(core._rows(t) for t in (B, C)), core._f32(D),
-                core._rows(z) if z is not None else None, core._f32(delta_bias))
-        init = core._f32(init)
-        out, fin, saved = core.selective_scan_forward(*args, softplus, init, seq, nseq, want_final, train)
-        if train:
-            ctx.softplus = softplus
-            ctx.save_for_backward(*args, init, seq, saved)
+        args, init = _layouts(u, delta, A, B, C, D, z, delta_bias), core._f32(init)
+        out, fin, saved = core.selective_scan_forward(*args, softplus, init, seq, nseq, want_final, True)
+        ctx.softplus = softplus
+        ctx.save_for_backward(*args, init, seq, saved)
         return out, fin
 
     @staticmethod
@@ -73,8 +75,12 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
     if cu is not None:
         core.require_cuda(u, cu)
         seq = core.sequence_index(cu, u.shape[1])
-    out, fin = SelectiveScan.apply(u, delta, A, B, C, D, z, delta_bias, initial_state, bool(delta_softplus), seq, nseq,
-                                   bool(return_final_state))
+    if core.training(u, delta, A, B, C, D, z, delta_bias, initial_state):
+        out, fin = SelectiveScan.apply(u, delta, A, B, C, D, z, delta_bias, initial_state, bool(delta_softplus), seq,
+                                       nseq, bool(return_final_state))
+    else:
+        out, fin, _ = core.selective_scan_forward(*_layouts(u, delta, A, B, C, D, z, delta_bias), bool(delta_softplus),
+                                                  core._f32(initial_state), seq, nseq, bool(return_final_state), False)
     return (out, fin) if return_final_state else out
 
 
