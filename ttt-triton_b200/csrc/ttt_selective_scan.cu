@@ -275,35 +275,38 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 3 : NPT == 8 ? 2 : 1) scan_chu
                    : static_cast<const T*>(p.B) + w.row * p.B_b + w.g * p.B_g;
   const long long r_l = REV ? p.C_l : p.B_l;
   float2 sum = all2(0.f);
-  for (int i = -1; i < ntiles; ++i) {
-    if (i + 1 < ntiles) {
-      const int tn = tile_at(i + 1);
-      auto& tile = s.tile[(i + 1) & 1];
-      Two<T> dd[F::TWOS], vv[F::TWOS], zz[F::TWOS];
-      Rows<T, F::NP, F::TT, F::HALF> rows;
+  Two<T> dd[F::TWOS], vv[F::TWOS], zz[F::TWOS];  // of the next tile, fetched an interval ahead
+  Rows<T, F::NP, F::TT, F::HALF> rows;
+  const auto fetch = [&](int i) {
+    const int tn = tile_at(i);
 #pragma unroll
-      for (int k = 0; k < F::TWOS; ++k) {
-        const int tok = tn + q.tq + k * F::STEP;
-        const bool in = tok < tend && in_sequence(seq, tok), on0 = in && q.on0, on1 = in && q.on1;
-        dd[k] = load_two(delta + tok * p.delta_l, on0, on1, p.couples);
-        vv[k] = load_two(v + tok * v_l, on0, on1, p.couples);
-        if (REV) zz[k] = load_two(z + tok * p.z_l, on0 && p.z, on1 && p.z, p.couples);
-      }
-      rows.fetch(q.tid, R, r_l, tn, tend, seq, p.quads);
-#pragma unroll
-      for (int k = 0; k < F::TWOS; ++k) {
-        const int t = q.tq + k * F::STEP, tok = tn + t;
-        float2 dt = __fadd2_rn(two_f(dd[k]), bias), x = two_f(vv[k]);
-        if (p.softplus) dt = softplus2(dt);
-        if (!(tok < tend && in_sequence(seq, tok))) dt = all2(0.f);
-        if (REV && p.z) x = __fmul2_rn(x, silu2(two_f(zz[k])));
-        if (!REV) x = __fmul2_rn(x, dt);
-        sum = __fadd2_rn(sum, dt);
-        *reinterpret_cast<float4*>(&tile.d[t * F::DT + q.pc]) = make_float4(dt.x, x.x, dt.y, x.y);
-      }
-      rows.put(q.tid, tile.B, R, r_l, tn, tend, p.N, seq, p.quads);
+    for (int k = 0; k < F::TWOS; ++k) {
+      const int tok = tn + q.tq + k * F::STEP;
+      const bool in = tok < tend && in_sequence(seq, tok), on0 = in && q.on0, on1 = in && q.on1;
+      dd[k] = load_two(delta + tok * p.delta_l, on0, on1, p.couples);
+      vv[k] = load_two(v + tok * v_l, on0, on1, p.couples);
+      if (REV) zz[k] = load_two(z + tok * p.z_l, on0 && p.z, on1 && p.z, p.couples);
     }
-    if (i + 1 < ntiles) tile_barrier();
+    rows.fetch(q.tid, R, r_l, tn, tend, seq, p.quads);
+  };
+  fetch(0);
+  for (int i = 0; i < ntiles; ++i) {  // prepares tile i while tile i - 1 runs
+    const int tn = tile_at(i);
+    auto& tile = s.tile[i & 1];
+#pragma unroll
+    for (int k = 0; k < F::TWOS; ++k) {
+      const int t = q.tq + k * F::STEP, tok = tn + t;
+      float2 dt = __fadd2_rn(two_f(dd[k]), bias), x = two_f(vv[k]);
+      if (p.softplus) dt = softplus2(dt);
+      if (!(tok < tend && in_sequence(seq, tok))) dt = all2(0.f);
+      if (REV && p.z) x = __fmul2_rn(x, silu2(two_f(zz[k])));
+      if (!REV) x = __fmul2_rn(x, dt);
+      sum = __fadd2_rn(sum, dt);
+      *reinterpret_cast<float4*>(&tile.d[t * F::DT + q.pc]) = make_float4(dt.x, x.x, dt.y, x.y);
+    }
+    rows.put(q.tid, tile.B, R, r_l, tn, tend, p.N, seq, p.quads);
+    if (i + 1 < ntiles) fetch(i + 1);
+    tile_barrier();
   }
   // the couples' threads have the step sizes' sums, one token in STEP each
   float* part = s.tile[0].y;
