@@ -51,9 +51,6 @@ __device__ __forceinline__ float softplus(float x) {
   q = fmaf(v, q, 2.f);
   return fmaf(s, q, fmaxf(x, 0.f));
 }
-// d/dx x sigmoid(x), given sigmoid(x)
-__device__ __forceinline__ float silu_grad(float x, float sg) { return sg * fmaf(x, 1.f - sg, 1.f); }
-
 // Packed rows: seq[t] is the sequence that token t belongs to, -1 for tokens of none. A token
 // whose predecessor belongs to another sequence starts its own, and likewise at the end.
 __device__ __forceinline__ bool seq_starts(const int* seq, int t) { return t == 0 || seq[t] != seq[t - 1]; }

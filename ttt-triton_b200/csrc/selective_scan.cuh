@@ -60,7 +60,6 @@ inline Shape shape_of(int N) {
 __host__ __device__ constexpr int save_every_of(int NPT) { return NPT == 16 ? 2 : 4; }
 inline int save_every(int N) { return save_every_of(shape_of(N).NPT); }
 
-
 // This thread's NPT states of channel d of a [.., D, N] array (0 past N); in fours where N is a
 // multiple of four and the array lies on a 16-byte boundary, as torch's allocations do.
 template <int NPT>
@@ -131,15 +130,6 @@ struct Rows {
     }
   }
 };
-// Both at once.
-template <typename T, int NP, int TT, int THREADS>
-__device__ __forceinline__ void stage_rows(float* dst, const T* src, long long ld, int t0, int t1, int N,
-                                           const int* seq, bool quads) {
-  Rows<T, NP, TT, THREADS> r;
-  r.fetch(threadIdx.x, src, ld, t0, t1, seq, quads);
-  r.put(threadIdx.x, dst, src, ld, t0, t1, N, seq, quads);
-}
-
 // Two adjacent channels of an activation. `both`: one access for the two, where every row has
 // them on a boundary of two; else each by itself, where it is there.
 template <typename T>
@@ -287,23 +277,6 @@ __device__ __forceinline__ float2 params_of(const float* v, int d, bool on0, boo
   return make_float2(v && on0 ? v[d] : 0.f, v && on1 ? v[d + 1] : 0.f);
 }
 
-// The sums over the LN threads of two adjacent channels.
-template <int LN>
-__device__ __forceinline__ float2 state_sums(const float* y) {
-  if constexpr (LN == 1) return *reinterpret_cast<const float2*>(y);
-  if constexpr (LN == 2) {
-    const float4 v = *reinterpret_cast<const float4*>(y);
-    return make_float2(v.x + v.y, v.z + v.w);
-  }
-  float2 r = make_float2(0.f, 0.f);
-#pragma unroll
-  for (int j = 0; j < LN / 4; ++j) {
-    const float4 v = reinterpret_cast<const float4*>(y)[j], x = reinterpret_cast<const float4*>(y + LN)[j];
-    r = __fadd2_rn(r, make_float2((v.x + v.y) + (v.z + v.w), (x.x + x.y) + (x.z + x.w)));
-  }
-  return r;
-}
-
 // exp(dt A) of a pair of states, A2 = A log2(e). The unit's 2^x cuts its argument off: for
 // arguments of -0.5 to -0.001 its results were 0.3 * 2^-24 too small on average, which a state
 // that is kept for a thousand tokens multiplies. Half a step of 2^-24 on the argument brings
@@ -330,18 +303,6 @@ __device__ __forceinline__ SeqMask warp_masks(const int* seq, int t0, int t1, in
   return m;
 }
 __device__ __forceinline__ bool in_sequence(const int* seq, int t) { return !seq || seq[t] >= 0; }
-template <int TT>
-__device__ __forceinline__ void stage_masks(SeqMask* m, const int* seq, int t0, int t1, int T) {
-  if (threadIdx.x < 32) {
-    const int t = t0 + threadIdx.x;
-    const bool on = threadIdx.x < TT && t < t1;
-    const unsigned s = __ballot_sync(0xffffffffu, on && seq_starts(seq, t));
-    const unsigned e = __ballot_sync(0xffffffffu, on && seq_ends(seq, t, T));
-    const unsigned v = __ballot_sync(0xffffffffu, on && seq[t] >= 0);
-    if (threadIdx.x == 0) m->start = s, m->end = e, m->in = v;
-  }
-}
-
 // Launches the pass over pieces (local end states, then the states entering each piece), when
 // the time axis is split. REV: the backward recurrence's carries instead of the states.
 int chunk_states(const Params& p, int dt, bool rev, cudaStream_t st, const char* who);

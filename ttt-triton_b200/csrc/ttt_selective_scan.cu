@@ -372,7 +372,7 @@ struct StepParams {
 // worked on: the state is read and written once, 8 N bytes a channel, and memory bounds it.
 template <typename T, int LN, int NPT, int ROWS>
 __global__ void __launch_bounds__(128) scan_step_kernel(const __grid_constant__ StepParams p) {
-  constexpr int DT = 128 / LN, H = NPT / 2;
+  constexpr int DT = 128 / LN;
   const int tid = threadIdx.x, nl = tid % LN, n0 = nl * NPT;
   const int tiles = (p.D + DT - 1) / DT;
   const int row0 = (int)(blockIdx.x / tiles) * ROWS, d = (int)(blockIdx.x % tiles) * DT + tid / LN;

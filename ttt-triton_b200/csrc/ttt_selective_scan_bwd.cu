@@ -37,7 +37,7 @@ int column_sum(const float* part, long long M, long long W, float* out, cudaStre
 static int channels_of_a_cta(int N) { return 256 / shape_of(N).LN; }  // Bwd::DT
 
 struct BwdScratch {
-  size_t tiles, part_bc, part_p, states;  // bytes but for tiles
+  size_t tiles, part_bc, part_p;  // bytes but for tiles
 };
 static BwdScratch bwd_scratch(int rows, int L, int D, int G, int N, int nchunks) {
   BwdScratch s;
