@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd.graph import increment_version
 
 from _core import _on_tensor_device
 from _lib import check, dtype_code, lib, require_cuda
@@ -231,6 +232,7 @@ def selective_scan_step(state, u, delta, A, B, C, D, z, delta_bias, softplus, in
     check(lib.ttt_selective_scan_step(rows, W, bs[1], N, state.shape[0], ptr(u), ptr(delta), ptr(B), ptr(C), ptr(z),
                                       dtype_code(u), st, ptr(A), ptr(D), ptr(delta_bias), int(softplus), ptr(index),
                                       ptr(state), ptr(out), stream_of(u)), "ttt_selective_scan_step")
+    increment_version(state)  # for autograd, as torch's own in-place operations do
     return out
 
 
@@ -318,4 +320,5 @@ def causal_conv_step(x, state, weight, bias, activation, index):
     check(lib.ttt_causal_conv_step(rows, W, K, state.shape[0], ptr(x), dtype_code(x),
                                    _strides(x.stride(0), state.stride(0)), ptr(w), ptr(b), act, ptr(index), ptr(state),
                                    ptr(y), stream_of(x)), "ttt_causal_conv_step")
+    increment_version(state)  # for autograd, as torch's own in-place operations do
     return y
