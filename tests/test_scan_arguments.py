@@ -1,0 +1,26 @@
+"""CPU: the argument checks of the selective scan and the causal convolution that come before
+any use of the device."""
+
+import pytest
+import torch
+
+import ops
+
+
+@pytest.mark.parametrize("dtype", [torch.complex64, torch.complex128])
+def test_complex_parameters_are_refused(dtype):
+    """A cast to fp32 would drop their imaginary part and compute another operator."""
+    x, A, B = torch.zeros(1, 4, 8), torch.zeros(8, 4), torch.zeros(1, 4, 4)
+    bad = lambda *shape: torch.ones(*shape, dtype=dtype)  # noqa: E731
+    for kw, name in ((dict(A=bad(8, 4)), "A"), (dict(D=bad(8)), "D"), (dict(delta_bias=bad(8)), "delta_bias"),
+                     (dict(initial_state=bad(1, 8, 4)), "initial_state")):
+        with pytest.raises(TypeError, match=f"{name} must be real"):
+            ops.selective_scan(x, x, kw.pop("A", A), B, B, **kw)
+    for kw, name in ((dict(A=bad(8, 4)), "A"), (dict(D=bad(8)), "D"), (dict(delta_bias=bad(8)), "delta_bias")):
+        with pytest.raises(TypeError, match=f"{name} must be real"):
+            ops.selective_scan_step(torch.zeros(1, 8, 4), x[:, 0], x[:, 0], kw.pop("A", A), B[:, 0], B[:, 0], **kw)
+    for w, b, name in ((bad(8, 3), None, "weight"), (torch.ones(8, 3), bad(8), "bias")):
+        with pytest.raises(TypeError, match=f"{name} must be real"):
+            ops.causal_conv1d(x, w, b)
+        with pytest.raises(TypeError, match=f"{name} must be real"):
+            ops.causal_conv1d_step(x[:, 0], torch.zeros(1, 2, 8), w, b)

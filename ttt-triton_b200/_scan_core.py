@@ -52,6 +52,14 @@ def _same(ref, **tensors):
             raise ValueError(f"{name} must have dtype {ref.dtype}, got {t.dtype}")
 
 
+def _real(**tensors):
+    """Parameters and states of other types are used in fp32, which would drop a complex one's
+    imaginary part."""
+    for name, t in tensors.items():
+        if isinstance(t, torch.Tensor) and t.is_complex():
+            raise TypeError(f"{name} must be real, got {t.dtype}")
+
+
 def _shaped(name, t, shape):
     if t is not None and t.shape != shape:
         raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
@@ -86,6 +94,7 @@ def packed(cu_seqlens, x):
 
 # --------------------------------------------------------------------------- selective scan
 def check_scan(u, delta, A, B, C, D, z, delta_bias, init, nseq):
+    _real(A=A, D=D, delta_bias=delta_bias, initial_state=init)
     require_cuda(*[t for t in (u, delta, A, B, C, D, z, delta_bias, init) if t is not None])
     dtype_code(u)
     if u.dim() != 3:
@@ -198,6 +207,7 @@ def _check_devices(tensors):
 @_on_tensor_device
 def selective_scan_step(state, u, delta, A, B, C, D, z, delta_bias, softplus, index):
     """One token per row: out [B, D]; state [slots, D, N] fp32 updated in place."""
+    _real(A=A, D=D, delta_bias=delta_bias)
     _check_devices((u, state, delta, A, B, C, D, z, delta_bias, index))
     shape = u.shape
     if len(shape) != 2:
@@ -251,6 +261,7 @@ def _check_taps(weight, bias, W):
 
 
 def check_conv(x, weight, bias, init, nseq):
+    _real(weight=weight, bias=bias)
     require_cuda(*(t for t in (x, weight, bias, init) if t is not None))
     dtype_code(x)
     if x.dim() != 3 or x.shape[2] < 1:
@@ -305,6 +316,7 @@ def causal_conv_backward(x, w, b, act, init, seq, dy, dfin, want_dinit):
 @_on_tensor_device
 def causal_conv_step(x, state, weight, bias, activation, index):
     """One token per row: y [B, D]; state [slots, K - 1, D] shifted in place."""
+    _real(weight=weight, bias=bias)
     _check_devices((x, state, weight, bias, index))
     act = _act_code(activation)
     if x.dim() != 2 or x.shape[1] < 1:
