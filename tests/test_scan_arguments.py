@@ -4,6 +4,7 @@ any use of the device."""
 import pytest
 import torch
 
+import _scan_core as core
 import ops
 
 
@@ -24,3 +25,20 @@ def test_complex_parameters_are_refused(dtype):
             ops.causal_conv1d(x, w, b)
         with pytest.raises(TypeError, match=f"{name} must be real"):
             ops.causal_conv1d_step(x[:, 0], torch.zeros(1, 2, 8), w, b)
+
+
+def test_state_layouts():
+    """Slots must be contiguous and apart; a dimension of one may have any stride."""
+    check = lambda state, shape: core._check_step(state, None, state.shape[0], (), shape)  # noqa: E731
+    wide = torch.zeros(3, 4, 8)
+    check(wide[:, 1:2], (1, 8))                           # one row of a longer window
+    check(torch.zeros(3, 8, 2)[:, :, :1].transpose(1, 2).transpose(1, 2)[:, :1], (1, 1))
+    check(torch.zeros(3, 8, 1), (8, 1))
+    check(torch.zeros(8, 3, 1).as_strided((3, 1, 8), (8, 3, 1)), (1, 8))
+    check(wide[:, 1:3], (2, 8))
+    check(torch.zeros(6, 4, 8)[::2], (4, 8))
+    for state, shape in ((wide[:, ::2], (2, 8)), (wide[..., :4], (4, 4)), (wide.transpose(1, 2), (8, 4)),
+                         (torch.zeros(3, 8, 2)[:, :, :1], (8, 1)), (torch.zeros(1, 1, 8).expand(3, 1, 8), (1, 8)),
+                         (torch.zeros(3, 1, 16)[..., ::2], (1, 8))):
+        with pytest.raises(ValueError):
+            check(state, shape)

@@ -55,3 +55,13 @@ def test_steps_in_inference_mode():
         rows = torch.zeros(2, 2, 8, device=DEV)
         ops.causal_conv1d_step(tok("u"), rows, torch.ones(8, 3, device=DEV))
         assert torch.equal(rows[:, 1], tok("u"))
+
+
+def test_a_step_on_one_row_of_a_longer_window():
+    """A two-tap filter's state as a slice of a wider one: that row is updated, the others are not."""
+    wide, x, w = (torch.randn(*s, device=DEV) for s in ((3, 4, 24), (3, 24), (24, 2)))
+    want, before = wide[:, 1:2].clone(), wide.clone()
+    y = ops.causal_conv1d_step(x, want, w)
+    assert torch.equal(ops.causal_conv1d_step(x, wide[:, 1:2], w), y)
+    assert torch.equal(wide[:, 1:2], want)
+    assert torch.equal(wide[:, [0, 2, 3]], before[:, [0, 2, 3]])

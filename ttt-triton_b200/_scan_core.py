@@ -184,7 +184,8 @@ def _check_step(state, index, rows, inputs, shape):
     size, stride = state.shape, state.stride()
     if len(size) != 3 or size[1:] != shape:
         raise ValueError(f"the state must be [slots, {shape[0]}, {shape[1]}], got {tuple(size)}")
-    if stride[2] != 1 or stride[1] != shape[1]:
+    # the stride of a dimension of one says nothing
+    if stride[2] != 1 and shape[1] > 1 or stride[1] != shape[1] and shape[0] > 1:
         raise ValueError("the state is updated in place: each slot must be contiguous")
     if size[0] > 1 and stride[0] < shape[0] * shape[1]:
         raise ValueError("the state's slots must not overlap")
