@@ -1,6 +1,8 @@
 """GPU: what a caller of the selective scan and the causal convolution may rely on beside their
 values at ordinary inputs."""
 
+import math
+
 import pytest
 import torch
 
@@ -10,6 +12,7 @@ from test_selective_scan_gpu import call, make
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 
 
 def on_device(t):
@@ -65,3 +68,46 @@ def test_a_step_on_one_row_of_a_longer_window():
     assert torch.equal(ops.causal_conv1d_step(x, wide[:, 1:2], w), y)
     assert torch.equal(wide[:, 1:2], want)
     assert torch.equal(wide[:, [0, 2, 3]], before[:, [0, 2, 3]])
+
+
+# ------------------------------------------------------------------------------ non-finite values
+def nonfinite_gradients(dtype, N, G, tensor, value, at, L=60):
+    """Gradients of a dense call with one non-finite value at token `at`, and of the same call
+    without it, on the device and from the 64-bit form."""
+    got = {}
+    for bad in (False, True):
+        t = make(1, L, 20, N, G, dtype, 12)
+        dy = torch.randn(1, L, 20, generator=torch.Generator().manual_seed(5)).to(dtype)
+        if bad:
+            (dy if tensor == "dy" else t[tensor])[0, at, 3] = value
+        leaves = {k: v.to(DEV).requires_grad_(True) for k, v in t.items()}
+        ref = {k: v.double().requires_grad_(True) for k, v in t.items()}
+        y = call(leaves, final=False)
+        ry, _ = R.selective_scan(*(ref[k] for k in ("u", "delta", "A", "B", "C", "D", "z", "bias")), True)
+        got[bad] = ([g.cpu() for g in torch.autograd.grad(y, [leaves[k] for k in ("B", "C")], dy.to(DEV))],
+                    torch.autograd.grad(ry, [ref[k] for k in ("B", "C")], dy.double()))
+    return got
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,G", [(3, 1), (8, 1), (16, 2), (32, 1), (40, 1), (100, 1)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("at", [0, 22, 25])
+def test_a_nonfinite_token_stays_out_of_its_neighbours_sums(dtype, N, G, value, at):
+    """dB and dC of the tokens that a non-finite input does not enter equal those without it: u
+    enters dB at its own token and dC from there on; dy enters dC at its own token and dB up
+    to there. Where an infinite product is the only one of its sum, the sum is that infinity."""
+    for tensor in ("u", "dy"):
+        runs = nonfinite_gradients(dtype, N, G, tensor, value, at)
+        (dB0, dC0), _ = runs[False]
+        (dB, dC), (rB, rC) = runs[True]
+        t = torch.arange(60)
+        cleanB, cleanC = (t != at, t < at) if tensor == "u" else (t > at, t != at)
+        assert torch.equal(dB[:, cleanB], dB0[:, cleanB]) and torch.equal(dC[:, cleanC], dC0[:, cleanC])
+        own = 0 if G == 1 else 3 // (20 // G)  # the group of channel 3
+        for g, r, clean in ((dB, rB, cleanB), (dC, rC, cleanC)):
+            assert not bool(torch.isfinite(g[0, at, own]).any())
+            if math.isinf(value):
+                r = r.to(dtype).float()
+                assert torch.equal(g[0, at, own].float().sign(), r[0, at, own].sign())
+                assert torch.equal(g[0, at].isnan(), r[0, at].isnan())

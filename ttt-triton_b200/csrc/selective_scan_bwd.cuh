@@ -49,6 +49,7 @@ struct Bwd {
     Tile tile[2];
     float2 dA[MAIN * NPT];                           // sums over many tiles
     float4 kept[RING][MAIN * NPT / 2];               // states before the coming runs, each thread's own
+    float4 carry[MAIN * NPT / 2];                    // what enters the run from behind, each thread's own
   };
 };
 
@@ -69,11 +70,14 @@ __device__ __forceinline__ float2 high2(float2 v) {
                      __uint_as_float(__float_as_uint(v.y) & 0xffffe000u));
 }
 // Adds a pair of states' v over the 4 threads of a channel group to the column that `one` marks.
-template <bool SPLIT>
+// CHECK: an infinite v has no low part (infinity less infinity is not a number).
+template <bool SPLIT, bool CHECK>
 __device__ __forceinline__ void add_over_channels(float (&c)[4], float2 v, float one) {
   if constexpr (SPLIT) {
     const float2 h = high2(v);
-    mma_16x8x4(c, high2(__fadd2_rn(v, neg2(h))), one);
+    float2 low = high2(__fadd2_rn(v, neg2(h)));
+    if constexpr (CHECK) low = make_float2(fabsf(h.x) < INFINITY ? low.x : 0.f, fabsf(h.y) < INFINITY ? low.y : 0.f);
+    mma_16x8x4(c, low, one);
     mma_16x8x4(c, h, one);
   } else {
     mma_16x8x4(c, make_float2(tf32(v.x), tf32(v.y)), one);
@@ -164,10 +168,14 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
       for (int t0 = tt + (F::RUNS - 1) * F::SUB; t0 >= tt; t0 -= F::SUB) {
         if (t0 >= tend) continue;
         const int b = t0 - tt;
-        const auto tokens = [&](auto checks) {
+        // The run's tokens. Without CHECK, whether its sums over channels are all finite: a product of
+        // several tokens has zeros in the columns of the others, and zero times a non-finite value
+        // spoils them. The run is then taken `again`, with a product for each token.
+        const auto tokens = [&](auto checks, bool again) {
           constexpr bool CHECK = decltype(checks)::value;
           float2 a[F::SUB][2][H], ah[F::SUB][2][H];
-          asm volatile("cp.async.wait_group %0;" ::"n"(F::RING - 2) : "memory");
+          float total = 0.f;
+          if (!again) asm volatile("cp.async.wait_group %0;" ::"n"(F::RING - 2) : "memory");
           Both<NPT> h;
 #pragma unroll
           for (int c = 0; c < 2; ++c)
@@ -176,8 +184,15 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
               const float4 q = s.kept[run % F::RING][tid + (c * (NPT / 4) + e) * F::MAIN];
               h.c[c].v[2 * e] = make_float2(q.x, q.y), h.c[c].v[2 * e + 1] = make_float2(q.z, q.w);
             }
-          fetch_states(run - (F::RING - 1));
-          --run;
+          if (!CHECK) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int e = 0; e < NPT / 4; ++e)
+                s.carry[tid + (c * (NPT / 4) + e) * F::MAIN] =
+                    make_float4(carry.c[c].v[2 * e].x, carry.c[c].v[2 * e].y, carry.c[c].v[2 * e + 1].x, carry.c[c].v[2 * e + 1].y);
+          }
+          if (!again) fetch_states(run - (F::RING - 1));
 #pragma unroll
           for (int k = 0; k < F::SUB; ++k) {
             if constexpr (CHECK && SEQ) {
@@ -197,7 +212,6 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
                 h.c[c].v[j] = __ffma2_rn(all2(c ? d4.w : d4.y), B2.v[j], ah[k][c][j]);
               }
           }
-          // tokens of two sequences never share a product: a NaN of one would reach the other's columns
           constexpr int TS = CHECK ? 1 : F::TS;
 #pragma unroll
           for (int g0 = F::SUB - TS; g0 >= 0; g0 -= TS) {
@@ -233,11 +247,11 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
                   s1[c] = j ? __ffma2_rn(g[c], B2.v[j], s1[c]) : __fmul2_rn(g[c], B2.v[j]);
                   s2[c] = j ? __ffma2_rn(q, A2.c[c].v[j], s2[c]) : __fmul2_rn(q, A2.c[c].v[j]);
                   s3[c] = j ? __ffma2_rn(hn[c], C2.v[j], s3[c]) : __fmul2_rn(hn[c], C2.v[j]);
-                  dA.c[c].v[j] = __ffma2_rn(q, all2(c ? d4.z : d4.x), dA.c[c].v[j]);
+                  if (!CHECK || !again) dA.c[c].v[j] = __ffma2_rn(q, all2(c ? d4.z : d4.x), dA.c[c].v[j]);
                   carry.c[c].v[j] = __fmul2_rn(a[k][c][j], g[c]);
                 }
-                add_over_channels<SPLIT>(accB[j], __ffma2_rn(g[0], all2(d4.y), __fmul2_rn(g[1], all2(d4.w))), one);
-                add_over_channels<SPLIT>(accC[j], __ffma2_rn(hn[0], all2(dy2.x), __fmul2_rn(hn[1], all2(dy2.y))), one);
+                add_over_channels<SPLIT, CHECK>(accB[j], __ffma2_rn(g[0], all2(d4.y), __fmul2_rn(g[1], all2(d4.w))), one);
+                add_over_channels<SPLIT, CHECK>(accC[j], __ffma2_rn(hn[0], all2(dy2.x), __fmul2_rn(hn[1], all2(dy2.y))), one);
               }
               const int o = ((b + k) * LN + nl) * F::YS + cl;
               *reinterpret_cast<float2*>(&tile.s1[o]) = make_float2(s1[0].x + s1[0].y, s1[1].x + s1[1].y);
@@ -249,6 +263,10 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
                   store_both<NPT>(p.dinit + sq * DN, d, n0, p.N, sq >= 0 && c0, sq >= 0 && c1, carry);
                 }
               }
+            }
+            if (!CHECK) {  // one of this lane's two columns: what is not finite is in all
+#pragma unroll
+              for (int j = 0; j < H; ++j) total += accB[j][0] + accB[j][2] + (accC[j][0] + accC[j][2]);
             }
             // of the products' two columns in this lane, those of the row's own channel group
 #pragma unroll
@@ -264,9 +282,22 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
               }
             }
           }
+          return fabsf(total) < INFINITY;
         };
-        if (t0 + F::SUB > tend || (SEQ && ((mask.start | mask.end) >> b & ((1u << F::SUB) - 1)))) tokens(std::true_type{});
-        else tokens(std::false_type{});
+        bool careful = t0 + F::SUB > tend || (SEQ && ((mask.start | mask.end) >> b & ((1u << F::SUB) - 1)));
+        bool again = false;
+        if (!careful && !__all_sync(0xffffffffu, tokens(std::false_type{}, false))) {
+          careful = again = true;
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int e = 0; e < NPT / 4; ++e) {
+              const float4 q = s.carry[tid + (c * (NPT / 4) + e) * F::MAIN];
+              carry.c[c].v[2 * e] = make_float2(q.x, q.y), carry.c[c].v[2 * e + 1] = make_float2(q.z, q.w);
+            }
+        }
+        if (careful) tokens(std::true_type{}, again);
+        --run;
       }
       if (i % 8 == 7 || i + 1 == ntiles) {  // short sums first: a long chain of additions loses bits
 #pragma unroll
