@@ -12,9 +12,9 @@
 // states (s1, s2 and y) pass through shared memory. Sums over channels (dB, dC): a thread adds
 // its two channels' products, and the tensor cores add over the threads, as products of the
 // matrix of those (16 states x 4 threads, one mma.sync a pair of states) with a vector of ones
-// in the column of the token and zeros in the others. The matrix has 11 bits there: for bf16
-// inputs the products are rounded to that (2^-11, against 2^-8 of dB's and dC's own type), for
-// fp16 and fp32 split in two such parts, 2^-21. What the CTAs of a group have of dB and dC, and
+// in the column of the token and zeros in the others. The matrix takes bf16 numbers: a summand is
+// the sum of two (bf16 inputs, rounded to 2^-17) or three (fp16 and fp32, exact), added in fp32.
+// What the CTAs of a group have of dB and dC, and
 // what the rows and pieces have of dA, dD and dbias, is written as partials and added in a
 // fixed order afterwards, so that results do not depend on timing.
 #pragma once
@@ -53,34 +53,33 @@ struct Bwd {
   };
 };
 
-__device__ __forceinline__ float tf32(float x) {
-  unsigned r;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-  return __uint_as_float(r);
-}
-// c += A b for the 16 x 4 matrix A with this thread's a in rows lane / 4 and 8 + lane / 4.
-__device__ __forceinline__ void mma_16x8x4(float (&c)[4], float2 a, float b) {
-  asm("mma.sync.aligned.m16n8k4.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(__float_as_uint(a.x)), "r"(__float_as_uint(a.y)), "r"(__float_as_uint(b)));
-}
-// The 11 leading bits of x, for the split form: x = high + high(x - high) to 2^-21.
-__device__ __forceinline__ float2 high2(float2 v) {
-  return make_float2(__uint_as_float(__float_as_uint(v.x) & 0xffffe000u),
-                     __uint_as_float(__float_as_uint(v.y) & 0xffffe000u));
-}
-// Adds a pair of states' v over the 4 threads of a channel group to the column that `one` marks.
-// CHECK: an infinite v has no low part (infinity less infinity is not a number).
-template <bool SPLIT, bool CHECK>
-__device__ __forceinline__ void add_over_channels(float (&c)[4], float2 v, float one) {
-  if constexpr (SPLIT) {
-    const float2 h = high2(v);
-    float2 low = high2(__fadd2_rn(v, neg2(h)));
-    if constexpr (CHECK) low = make_float2(fabsf(h.x) < INFINITY ? low.x : 0.f, fabsf(h.y) < INFINITY ? low.y : 0.f);
-    mma_16x8x4(c, low, one);
-    mma_16x8x4(c, h, one);
+// Adds a pair of states' v over the 4 threads of a channel group to the column that `one` (two
+// bf16 ones, or zeros) marks. A value is the sum of bf16 numbers, its leading 8 bits, the next 8
+// and the rest, which the matrix takes as terms of their own: a thread has columns
+// 2 (lane % 4), + 1 (+ 8, + 9) of row lane / 4 for v.x and of 8 + lane / 4 for v.y.
+// EXACT: three parts, all 24 bits. Else two, the second rounded: 2^-17 of a value, which is 2^-8 of
+// the half step that dB and dC of bf16 inputs are rounded by (16 x 2048 x 1536, 16 states:
+// backward 1.27 ms, 1.55 ms with three parts). CHECK: an infinite v has no further parts (infinity less
+// infinity is not a number).
+template <bool EXACT, bool CHECK>
+__device__ __forceinline__ void add_over_channels(float (&c)[4], float2 v, unsigned one) {
+  const auto lead = [](float2 x) {
+    return make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffff0000u), __uint_as_float(__float_as_uint(x.y) & 0xffff0000u));
+  };
+  const auto both = [](float x, unsigned r) { return __byte_perm(__float_as_uint(x), r, 0x7632); };  // the two leads
+  const float2 h = lead(v);
+  float2 r = __ffma2_rn(h, all2(-1.f), v);
+  if constexpr (CHECK) r = make_float2(fabsf(h.x) < INFINITY ? r.x : 0.f, fabsf(h.y) < INFINITY ? r.y : 0.f);
+  if constexpr (EXACT) {
+    const float2 l = __ffma2_rn(lead(r), all2(-1.f), r);
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%8}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(both(v.x, __float_as_uint(r.x))), "r"(both(v.y, __float_as_uint(r.y))), "r"(__float_as_uint(l.x)),
+          "r"(__float_as_uint(l.y)), "r"(one));
   } else {
-    mma_16x8x4(c, make_float2(tf32(v.x), tf32(v.y)), one);
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(both(v.x, __float_as_uint(r.x) + 0x8000u)), "r"(both(v.y, __float_as_uint(r.y) + 0x8000u)), "r"(one));
   }
 }
 
@@ -93,7 +92,7 @@ __device__ __forceinline__ void part_barrier() {
 template <typename T, int LN, int NPT, bool SEQ, bool TWO>
 __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const __grid_constant__ Params p) {
   using F = Bwd<LN, NPT>;
-  constexpr bool SPLIT = !std::is_same<T, __nv_bfloat16>::value;
+  constexpr bool EXACT = !std::is_same<T, __nv_bfloat16>::value;
   constexpr int H = NPT / 2;
   extern __shared__ __align__(16) unsigned char raw_smem[];
   auto& s = *reinterpret_cast<typename F::Smem*>(raw_smem);
@@ -232,7 +231,7 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
               const float4 d4 = *reinterpret_cast<const float4*>(&tile.d[(b + k) * F::DT + cl]);
               const float2 dy2 = *reinterpret_cast<const float2*>(&tile.dy[(b + k) * F::DT + cl]);
               const Pairs<NPT> B2 = row_pairs<NPT>(tile.B + (b + k) * F::NP + n0), C2 = row_pairs<NPT>(tile.C + (b + k) * F::NP + n0);
-              const float one = col_tok == k - g0 ? 1.f : 0.f;
+              const unsigned one = col_tok == k - g0 ? 0x3f803f80u : 0u;
               const float2 zero = all2(0.f);
               float2 s1[2] = {zero, zero}, s2[2] = {zero, zero}, s3[2] = {zero, zero};
 #pragma unroll
@@ -250,8 +249,8 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
                   if (!CHECK || !again) dA.c[c].v[j] = __ffma2_rn(q, all2(c ? d4.z : d4.x), dA.c[c].v[j]);
                   carry.c[c].v[j] = __fmul2_rn(a[k][c][j], g[c]);
                 }
-                add_over_channels<SPLIT, CHECK>(accB[j], __ffma2_rn(g[0], all2(d4.y), __fmul2_rn(g[1], all2(d4.w))), one);
-                add_over_channels<SPLIT, CHECK>(accC[j], __ffma2_rn(hn[0], all2(dy2.x), __fmul2_rn(hn[1], all2(dy2.y))), one);
+                add_over_channels<EXACT, CHECK>(accB[j], __ffma2_rn(g[0], all2(d4.y), __fmul2_rn(g[1], all2(d4.w))), one);
+                add_over_channels<EXACT, CHECK>(accC[j], __ffma2_rn(hn[0], all2(dy2.x), __fmul2_rn(hn[1], all2(dy2.y))), one);
               }
               const int o = ((b + k) * LN + nl) * F::YS + cl;
               *reinterpret_cast<float2*>(&tile.s1[o]) = make_float2(s1[0].x + s1[0].y, s1[1].x + s1[1].y);
