@@ -60,7 +60,8 @@ struct Bwd {
 // EXACT: three parts, all 24 bits. Else two, the second rounded: 2^-17 of a value, which is 2^-8 of
 // the half step that dB and dC of bf16 inputs are rounded by (16 x 2048 x 1536, 16 states:
 // backward 1.27 ms, 1.55 ms with three parts). CHECK: an infinite v has no further parts (infinity less
-// infinity is not a number).
+// infinity is not a number). The products are volatile: all 32 lanes have to execute them, and what
+// follows stores their results in some lanes only, where the compiler could otherwise move them.
 template <bool EXACT, bool CHECK>
 __device__ __forceinline__ void add_over_channels(float (&c)[4], float2 v, unsigned one) {
   const auto lead = [](float2 x) {
@@ -72,12 +73,12 @@ __device__ __forceinline__ void add_over_channels(float (&c)[4], float2 v, unsig
   if constexpr (CHECK) r = make_float2(fabsf(h.x) < INFINITY ? r.x : 0.f, fabsf(h.y) < INFINITY ? r.y : 0.f);
   if constexpr (EXACT) {
     const float2 l = __ffma2_rn(lead(r), all2(-1.f), r);
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%8}, {%0,%1,%2,%3};"
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%8}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(both(v.x, __float_as_uint(r.x))), "r"(both(v.y, __float_as_uint(r.y))), "r"(__float_as_uint(l.x)),
           "r"(__float_as_uint(l.y)), "r"(one));
   } else {
-    asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(both(v.x, __float_as_uint(r.x) + 0x8000u)), "r"(both(v.y, __float_as_uint(r.y) + 0x8000u)), "r"(one));
   }
