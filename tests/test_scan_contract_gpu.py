@@ -129,3 +129,24 @@ def test_bf16_sums_over_channels_round_as_fp32_ones():
     want = torch.autograd.grad(ry, [ref["B"], ref["C"]], dy.double())
     for g, w in zip(got, want):
         assert float((g.cpu() != w.bfloat16()).double().mean()) <= 5e-3
+
+
+# ------------------------------------------------------------------------------ long sums
+@pytest.mark.parametrize("N", [1, 8, 16])
+def test_sums_over_long_rows(N):
+    """dD = sum u dy and dbias = sum ddelta over 256 rows of 20000 equal tokens, which are not split
+    (the rows fill the device), against 64-bit sums of the same fp32 terms. Adding n terms of one
+    sign one after another is off by n / 2 half steps of 2^-24 at worst, and equal terms come near
+    that. A thread's sums are of at most 32 terms, 20000 / 32 of which are added in turn, and the
+    rows' sum is of 16 and 16: 16 + 313 + 16."""
+    B, L, D = 256, 20000, 4
+    full = lambda *s, v: torch.full(s, v, device=DEV)  # noqa: E731
+    t = {"u": full(B, L, D, v=1 / 3), "delta": full(B, L, D, v=0.05), "A": -torch.arange(1, N + 1, device=DEV).expand(D, N).float(),
+         "B": full(B, L, 1, N, v=0.7), "C": full(B, L, 1, N, v=0.3), "D": full(D, v=1.0), "bias": full(D, v=0.0)}
+    leaves = {k: t[k].requires_grad_(True) for k in ("delta", "D", "bias")}
+    y = call(t, softplus=False, final=False)
+    dy = full(B, L, D, v=0.1)
+    ddelta, dD, dbias = torch.autograd.grad(y, list(leaves.values()), dy)
+    for got, terms in ((dD, t["u"].double() * dy.double()), (dbias, ddelta.double())):
+        want = terms.sum((0, 1))
+        assert float(((got.double() - want) / want).abs().max()) <= (16 + 313 + 16) * 2.0**-24

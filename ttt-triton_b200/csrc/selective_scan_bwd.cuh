@@ -47,7 +47,7 @@ struct Bwd {
   };
   struct Smem {
     Tile tile[2];
-    float2 dA[MAIN * NPT];                           // sums over many tiles
+    float2 dA[MAIN * NPT], dD[HELP], dbias[HELP];    // sums over many tiles
     float4 kept[RING][MAIN * NPT / 2];               // states before the coming runs, each thread's own
     float4 carry[MAIN * NPT / 2];                    // what enters the run from behind, each thread's own
   };
@@ -317,7 +317,6 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
 #pragma unroll
       for (int j = 0; j < H; ++j) dA.c[c].v[j] = s.dA[tid + (c * H + j) * F::MAIN];
     store_both<NPT>(part, d, n0, p.N, c0, c1, dA);
-    part_barrier<1, F::THREADS>();
     return;
   }
 
@@ -328,6 +327,7 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
   const bool on0 = w.d0 + pc < p.Dg, on1 = w.d0 + pc + 1 < p.Dg;
   const float2 skip = params_of(p.Dskip, pd, on0, on1), bias = params_of(p.bias, pd, on0, on1);
   float2 sum_D = all2(0.f), sum_bias = sum_D;
+  s.dD[tid] = s.dbias[tid] = sum_D;
   const long long row0 = (long long)w.row * p.L, t_last = (long long)last * F::TB + tq;
   const T* u = static_cast<const T*>(p.u) + w.row * p.u_b + t_last * p.u_l + pd;
   const T* delta = static_cast<const T*>(p.delta) + w.row * p.delta_b + t_last * p.delta_l + pd;
@@ -413,6 +413,10 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
         }
       }
       part_B -= F::TB * part_step, part_C -= F::TB * part_step;
+      if (i % 8 == 0 || i == ntiles) {  // short sums first, as for dA
+        s.dD[tid] = __fadd2_rn(s.dD[tid], sum_D), s.dbias[tid] = __fadd2_rn(s.dbias[tid], sum_bias);
+        sum_D = sum_bias = all2(0.f);
+      }
     }
 #pragma unroll
     for (int k = 0; k < F::TWOS; ++k) r0[k] = r1[k], r1[k] = r2[k];
@@ -436,21 +440,14 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
     if (i < ntiles) part_barrier<1, F::THREADS>();
   }
 
-  // the couples' sums over their tokens; both parts are done with the tiles
-  part_barrier<1, F::THREADS>();
-  float2* red = reinterpret_cast<float2*>(s.tile[0].s1);
+  part_barrier<2, F::HELP>();
+  if (tq == 0) {  // the couples' sums over their tokens
+    float2 dD = s.dD[tid], dbias = s.dbias[tid];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    float2 v = k ? sum_bias : sum_D;
-    red[k * F::HELP + tid] = v;
-    part_barrier<2, F::HELP>();
-    if (tq == 0) {
-#pragma unroll
-      for (int j = 1; j < F::STEP; ++j) v = __fadd2_rn(v, red[k * F::HELP + tid + j * (F::DT / 2)]);
-      const long long o = DN + (long long)k * p.D + pd;
-      if (on0) part[o] = v.x;
-      if (on1) part[o + 1] = v.y;
-    }
+    for (int j = 1; j < F::STEP; ++j)
+      dD = __fadd2_rn(dD, s.dD[tid + j * (F::DT / 2)]), dbias = __fadd2_rn(dbias, s.dbias[tid + j * (F::DT / 2)]);
+    if (on0) part[DN + pd] = dD.x, part[DN + p.D + pd] = dbias.x;
+    if (on1) part[DN + pd + 1] = dD.y, part[DN + p.D + pd + 1] = dbias.y;
   }
 }
 
