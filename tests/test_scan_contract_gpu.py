@@ -150,3 +150,45 @@ def test_sums_over_long_rows(N):
     for got, terms in ((dD, t["u"].double() * dy.double()), (dbias, ddelta.double())):
         want = terms.sum((0, 1))
         assert float(((got.double() - want) / want).abs().max()) <= (16 + 313 + 16) * 2.0**-24
+
+
+# ------------------------------------------------------------------------------ autograd
+def test_gradients_of_a_graph_and_of_casts():
+    """With create_graph the gradients are the same and have none themselves (torch's once_differentiable
+    says so where the upstream gradient has one); parameters in 16 bits and transposed inputs
+    get gradients of their own type and order."""
+    t = on_device(make(2, 12, 8, 4, 1, torch.float32, 3))
+    x, A = t["u"].requires_grad_(True), t["A"].requires_grad_(True)
+    w = torch.randn(8, 3, device=DEV).bfloat16().requires_grad_(True)
+    b = torch.randn(8, device=DEV).half().requires_grad_(True)
+    xt = t["z"].transpose(1, 2).contiguous().transpose(1, 2).requires_grad_(True)
+    for f, leaves in ((lambda: call(t, final=False), [x, A]),
+                      (lambda: ops.causal_conv1d(x, w, b, "silu"), [x, w, b]),
+                      (lambda: ops.causal_conv1d(xt, w, b, "silu"), [xt, w, b])):
+        y = f()
+        dy = torch.randn_like(y)
+        plain = torch.autograd.grad(y, leaves, dy)
+        graph = torch.autograd.grad(f(), leaves, dy.clone().requires_grad_(True), create_graph=True)
+        assert all(torch.equal(p, g) and p.dtype == v.dtype for p, g, v in zip(plain, graph, leaves))
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            graph[0].float().sum().backward()
+    want = torch.autograd.grad(ops.causal_conv1d(xt.detach().contiguous().requires_grad_(True), w, b, "silu"), [w, b], dy)
+    assert all(torch.equal(p, q) for p, q in zip(plain[1:], want))
+
+
+def test_an_output_or_a_final_state_alone():
+    """Gradients where only one of the two outputs has one."""
+    t = on_device(make(2, 12, 8, 4, 1, torch.float32, 3, 2))
+    leaves = {k: v.requires_grad_(True) for k, v in t.items()}
+    both = lambda: call(leaves)  # noqa: E731
+    conv_init = torch.randn(2, 2, 8, device=DEV, requires_grad=True)
+    w = torch.randn(8, 3, device=DEV, requires_grad=True)
+    conv = lambda: ops.causal_conv1d(leaves["u"], w, None, "silu", conv_init, None, True)  # noqa: E731
+    for f, ins in ((both, list(leaves.values())), (conv, [leaves["u"], w, conv_init])):
+        y, fin = f()
+        dy, df = torch.randn_like(y), torch.randn_like(fin)
+        sums = torch.autograd.grad([y, fin], ins, [dy, df])
+        alone = (torch.autograd.grad(f()[i], ins, g, allow_unused=True) for i, g in enumerate((dy, df)))
+        for s, p, q in zip(sums, *alone):
+            p, q = (torch.zeros_like(s) if v is None else v for v in (p, q))
+            assert R.rel(p + q, s) <= 2.0**-20

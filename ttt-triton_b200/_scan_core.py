@@ -8,19 +8,36 @@ dimension is contiguous; others are copied. Nothing here synchronises the device
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
+from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
-from _core import _on_tensor_device
-from _lib import check, dtype_code, lib, require_cuda
+from _lib import DTYPE_CODES, check, dtype_code, lib, require_cuda
 
 MAX_STATES = 128
 
 
-# These calls are short: for a single token the host's work is most of their time. Addresses go
-# to ctypes as plain integers, and the current stream is asked for without wrapping it.
+# These calls are short: the host's work is most of the time of a single token, and of a small
+# training call, whose backward runs in a thread of autograd's with cold caches. Addresses go to
+# ctypes as plain integers, and the current device and stream are asked for without wrapping them.
 _current_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
+def _on_device(fn):
+    """Runs a function with its first argument's device current, as ``_core._on_tensor_device``."""
+
+    @functools.wraps(fn)
+    def wrapper(t, *args):
+        dev = t.get_device()
+        if dev < 0 or dev == _current_device():
+            return fn(t, *args)
+        with torch.cuda.device(dev):
+            return fn(t, *args)
+
+    return wrapper
 
 
 def ptr(t):
@@ -36,8 +53,25 @@ def _rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _check_devices(tensors):
+    """All of them on one CUDA device."""
+    try:
+        dev = tensors[0].get_device()
+        for t in tensors:
+            if t is not None and t.get_device() != dev or dev < 0:
+                break
+        else:
+            return
+    except AttributeError:
+        pass
+    require_cuda(*(t for t in tensors if t is not None))
+
+
 def _strides(*values):
     return (ctypes.c_longlong * len(values))(*values)
+
+
+_Strides2 = ctypes.c_longlong * 2
 
 
 def _f32(t):
@@ -46,18 +80,40 @@ def _f32(t):
     return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
 
 
+def _as(t, dtype):
+    return t if t.dtype is dtype else t.to(dtype)
+
+
+def _upstream(grad, ref):
+    """An output's gradient, of the type of ref and contiguous; zero where there is none."""
+    if grad is None:
+        return torch.zeros(ref.shape, device=ref.device, dtype=ref.dtype)
+    return grad if grad.dtype is ref.dtype and grad.is_contiguous() else grad.to(ref.dtype).contiguous()
+
+
+def first_order(backward):
+    """A backward whose gradients have none themselves: ``once_differentiable``, whose wrapping is
+    left out where no graph is recorded."""
+    guarded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def wrapper(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return wrapper
+
+
 def _same(ref, **tensors):
     for name, t in tensors.items():
         if t is not None and t.dtype != ref.dtype:
             raise ValueError(f"{name} must have dtype {ref.dtype}, got {t.dtype}")
 
 
-def _real(**tensors):
+def _real(name, t):
     """Parameters and states of other types are used in fp32, which would drop a complex one's
     imaginary part."""
-    for name, t in tensors.items():
-        if isinstance(t, torch.Tensor) and t.is_complex():
-            raise TypeError(f"{name} must be real, got {t.dtype}")
+    if isinstance(t, torch.Tensor) and t.dtype is not torch.float32 and t.is_complex():
+        raise TypeError(f"{name} must be real, got {t.dtype}")
 
 
 def _shaped(name, t, shape):
@@ -65,7 +121,7 @@ def _shaped(name, t, shape):
         raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
 
 
-@_on_tensor_device
+@_on_device
 def sequence_index(cu_seqlens, T):
     """Each token's sequence, int32 [T], from S + 1 ascending offsets; -1 outside of all."""
     seq = torch.empty(T, device=cu_seqlens.device, dtype=torch.int32)
@@ -78,13 +134,15 @@ def sequence_index(cu_seqlens, T):
 def training(*tensors):
     """Whether a call has a gradient to prepare for. (Inside an autograd function's forward both
     the mode and the inputs' flags say something else.)"""
-    return torch.is_grad_enabled() and any([t.requires_grad for t in tensors if t is not None])
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def packed(cu_seqlens, x):
-    """(number of sequences, checked int32 offsets) of a batch of shape x.shape[:2]."""
-    if cu_seqlens is None:
-        return x.shape[0], None
+    """(number of sequences, checked int32 offsets) of a row of packed sequences."""
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.is_floating_point():
         raise ValueError("cu_seqlens must hold the S + 1 >= 2 offsets of S packed sequences")
     if x.shape[0] != 1:
@@ -94,8 +152,8 @@ def packed(cu_seqlens, x):
 
 # --------------------------------------------------------------------------- selective scan
 def check_scan(u, delta, A, B, C, D, z, delta_bias, init, nseq):
-    _real(A=A, D=D, delta_bias=delta_bias, initial_state=init)
-    require_cuda(*[t for t in (u, delta, A, B, C, D, z, delta_bias, init) if t is not None])
+    _real("A", A), _real("D", D), _real("delta_bias", delta_bias), _real("initial_state", init)
+    _check_devices((u, delta, A, B, C, D, z, delta_bias, init))
     dtype_code(u)
     if u.dim() != 3:
         raise ValueError(f"u must be [B, L, D], got shape {tuple(u.shape)}")
@@ -127,7 +185,7 @@ def _scan_args(u, delta, A, B, C, D, z, delta_bias, softplus):
             ptr(D), ptr(delta_bias), int(softplus))
 
 
-@_on_tensor_device
+@_on_device
 def selective_scan_forward(u, delta, A, B, C, D, z, delta_bias, softplus, init, seq, nseq, want_final, for_backward):
     """Returns (out [B, L, D] in u's dtype, final state fp32 or None, saved states or None).
     u, delta, B, C, z with contiguous last dimensions; A, D, delta_bias, init fp32 contiguous."""
@@ -153,7 +211,7 @@ def selective_scan_forward(u, delta, A, B, C, D, z, delta_bias, softplus, init, 
     return out, fin, saved
 
 
-@_on_tensor_device
+@_on_device
 def selective_scan_backward(u, delta, A, B, C, D, z, delta_bias, softplus, init, seq, saved, dout, dfin, want_dinit):
     """Returns (du, ddelta, dA, dB, dC, dD, dz or None, ddelta_bias, dinit or None); the
     gradients of A, D, delta_bias and the state in fp32, the others in u's dtype."""
@@ -162,7 +220,8 @@ def selective_scan_backward(u, delta, A, B, C, D, z, delta_bias, softplus, init,
     dev, dt = u.device, u.dtype
     du, ddelta = torch.empty_like(dout), torch.empty_like(dout)
     dz = torch.empty_like(dout) if z is not None else None
-    dB, dC = torch.empty(2, rows, L, G, N, device=dev, dtype=dt).unbind(0)
+    dB = torch.empty(rows, L, G, N, device=dev, dtype=dt)
+    dC = torch.empty_like(dB)
     dinit = None
     if want_dinit:
         dinit = dfin.clone() if dfin is not None else torch.zeros(init.shape, device=dev, dtype=torch.float32)
@@ -176,7 +235,9 @@ def selective_scan_backward(u, delta, A, B, C, D, z, delta_bias, softplus, init,
                                      ptr(saved), ptr(dout), ptr(dfin), ptr(du), ptr(ddelta), ptr(dB), ptr(dC), ptr(dz),
                                      ptr(dinit), ptr(dparams), ptr(scratch), nbytes, stream_of(u)),
           "ttt_selective_scan_bwd")
-    return du, ddelta, dparams[:W * N].view(W, N), dB, dC, dparams[W * N:W * (N + 1)], dz, dparams[W * (N + 1):], dinit
+    dA, dD, dbias = (dparams.as_strided((W, N), (N, 1)), dparams.as_strided((W,), (1,), W * N),
+                     dparams.as_strided((W,), (1,), W * (N + 1)))
+    return du, ddelta, dA, dB, dC, dD, dz, dbias, dinit
 
 
 def _check_step(state, index, rows, inputs, shape):
@@ -198,17 +259,10 @@ def _check_step(state, index, rows, inputs, shape):
         raise RuntimeError("the single-token step has no gradient: call it under torch.no_grad()")
 
 
-def _check_devices(tensors):
-    dev = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and t.get_device() != dev or dev < 0:
-            require_cuda(*(t for t in tensors if t is not None))
-
-
-@_on_tensor_device
+@_on_device
 def selective_scan_step(state, u, delta, A, B, C, D, z, delta_bias, softplus, index):
     """One token per row: out [B, D]; state [slots, D, N] fp32 updated in place."""
-    _real(A=A, D=D, delta_bias=delta_bias)
+    _real("A", A), _real("D", D), _real("delta_bias", delta_bias)
     _check_devices((u, state, delta, A, B, C, D, z, delta_bias, index))
     shape = u.shape
     if len(shape) != 2:
@@ -255,69 +309,93 @@ def _act_code(activation):
 
 
 def _check_taps(weight, bias, W):
-    if weight.dim() != 2 or weight.shape[0] != W or not 2 <= weight.shape[1] <= 4:
-        raise ValueError(f"weight must be [{W}, K] with 2 to 4 taps, got {tuple(weight.shape)}")
+    shape = weight.shape
+    if len(shape) != 2 or shape[0] != W or not 2 <= shape[1] <= 4:
+        raise ValueError(f"weight must be [{W}, K] with 2 to 4 taps, got {tuple(shape)}")
     _shaped("bias", bias, (W,))
-    return weight.shape[1]
+    return shape[1]
+
+
+def _conv_sizes(x, weight, bias, init, nseq):
+    """(rows, L, D, K, type code) of a call, or what is wrong with it."""
+    if x.dim() != 3:
+        raise ValueError(f"x must be [B, L, D], got shape {tuple(x.shape)}")
+    _real("weight", weight), _real("bias", bias)
+    _check_devices((x, weight, bias, init))
+    dt, shape = dtype_code(x), x.shape
+    if shape[2] < 1:
+        raise ValueError(f"x must be [B, L, D], got shape {tuple(shape)}")
+    K = _check_taps(weight, bias, shape[2])
+    _shaped("initial_state", init, (nseq, K - 1, shape[2]))
+    _same(x, initial_state=init)
+    return (*shape, K, dt)
 
 
 def check_conv(x, weight, bias, init, nseq):
-    _real(weight=weight, bias=bias)
-    require_cuda(*(t for t in (x, weight, bias, init) if t is not None))
-    dtype_code(x)
-    if x.dim() != 3 or x.shape[2] < 1:
-        raise ValueError(f"x must be [B, L, D], got shape {tuple(x.shape)}")
-    W = x.shape[2]
-    K = _check_taps(weight, bias, W)
-    _shaped("initial_state", init, (nseq, K - 1, W))
-    _same(x, initial_state=init)
-    return K
+    """The same; a call with nothing but plain parameters is seen to be right at a glance."""
+    f32 = torch.float32
+    if init is None and weight.dtype is f32 and (bias is None or bias.dtype is f32):
+        dev, size, taps = x.get_device(), x.shape, weight.shape
+        if (dev >= 0 and weight.get_device() == dev and len(size) == 3 and len(taps) == 2 and size[2] == taps[0] > 0
+                and 2 <= taps[1] <= 4 and (bias is None or bias.get_device() == dev and bias.shape == taps[:1])
+                and x.dtype in DTYPE_CODES):
+            return (*size, taps[1], DTYPE_CODES[x.dtype])
+    return _conv_sizes(x, weight, bias, init, nseq)
 
 
-@_on_tensor_device
-def causal_conv_forward(x, w, b, act, init, seq, nseq, want_final):
-    """Returns (y [B, L, D], final state [sequences, K - 1, D] or None), both in x's dtype."""
-    rows, L, W = x.shape
-    K = w.shape[1]
-    y = torch.empty(rows, L, W, device=x.device, dtype=x.dtype)
+def causal_conv_forward(x, w, b, act, init, seq, nseq, want_final, sizes, for_backward):
+    """Returns (y [B, L, D], final state [sequences, K - 1, D] or None), both in x's dtype, and the
+    bytes of scratch of the backward (0 without one)."""
+    dev = x.get_device()
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return causal_conv_forward(x, w, b, act, init, seq, nseq, want_final, sizes, for_backward)
+    rows, L, W, K, dt = sizes
+    y = torch.empty_like(x) if x.is_contiguous() else x.new_empty((rows, L, W))
     fin = None
     if want_final:
         if seq is None and L:
-            fin = torch.empty(nseq, K - 1, W, device=x.device, dtype=x.dtype)
+            fin = x.new_empty((nseq, K - 1, W))
         else:
-            fin = init.clone() if init is not None else torch.zeros(nseq, K - 1, W, device=x.device, dtype=x.dtype)
+            fin = init.clone() if init is not None else x.new_zeros((nseq, K - 1, W))
     if rows * L == 0:
-        return y, fin
-    check(lib.ttt_causal_conv_fwd(rows, L, W, K, ptr(x), dtype_code(x), _strides(x.stride(0), x.stride(1)), ptr(w),
-                                  ptr(b), act, ptr(seq), ptr(init), ptr(fin), ptr(y), stream_of(x)),
-          "ttt_causal_conv_fwd")
-    return y, fin
+        return y, fin, 0
+    st = x.stride()
+    rc = lib.ttt_causal_conv_fwd(rows, L, W, K, x.data_ptr(), dt, _Strides2(st[0], st[1]), w.data_ptr(), ptr(b), act,
+                                 ptr(seq), ptr(init), ptr(fin), y.data_ptr(), _current_stream(dev))
+    if rc:
+        check(rc, "ttt_causal_conv_fwd")
+    return y, fin, lib.ttt_causal_conv_bwd_scratch_bytes(*sizes) if for_backward else 0
 
 
-@_on_tensor_device
-def causal_conv_backward(x, w, b, act, init, seq, dy, dfin, want_dinit):
-    """Returns (dx, dw fp32, db fp32, dinit or None)."""
-    rows, L, W = x.shape
-    K = w.shape[1]
-    dx = torch.empty(rows, L, W, device=x.device, dtype=x.dtype)
+def causal_conv_backward(x, w, b, act, init, seq, dy, dfin, want_dinit, sizes, nbytes):
+    """Returns (dx, dw fp32, db fp32, dinit or None); dy of x's dtype and contiguous, nbytes as the
+    forward gave them."""
+    dev = x.get_device()
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return causal_conv_backward(x, w, b, act, init, seq, dy, dfin, want_dinit, sizes, nbytes)
+    rows, L, W, K, dt = sizes
+    dx = torch.empty_like(dy)
     dinit = None
     if want_dinit:
-        dinit = dfin.clone() if dfin is not None else torch.zeros(init.shape, device=x.device, dtype=x.dtype)
+        dinit = dfin.clone() if dfin is not None else torch.zeros_like(init)
     if rows * L == 0:
-        return dx, torch.zeros_like(w), torch.zeros(W, device=x.device, dtype=torch.float32), dinit
-    dparams = torch.empty(W * (K + 1), device=x.device, dtype=torch.float32)
-    nbytes = lib.ttt_causal_conv_bwd_scratch_bytes(rows, L, W, K, dtype_code(x))
-    scratch = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
-    check(lib.ttt_causal_conv_bwd(rows, L, W, K, ptr(x), dtype_code(x), _strides(x.stride(0), x.stride(1)), ptr(w),
-                                  ptr(b), act, ptr(seq), ptr(init), ptr(dy), ptr(dfin), ptr(dx), ptr(dinit),
-                                  ptr(dparams), ptr(scratch), nbytes, stream_of(x)), "ttt_causal_conv_bwd")
-    return dx, dparams[:W * K].view(W, K), dparams[W * K:], dinit
+        return dx, torch.zeros_like(w), w.new_zeros(W), dinit
+    dparams, scratch = w.new_empty(W * (K + 1)), w.new_empty(nbytes // 4)
+    st = x.stride()
+    rc = lib.ttt_causal_conv_bwd(rows, L, W, K, x.data_ptr(), dt, _Strides2(st[0], st[1]), w.data_ptr(), ptr(b), act,
+                                 ptr(seq), ptr(init), dy.data_ptr(), ptr(dfin), dx.data_ptr(), ptr(dinit),
+                                 dparams.data_ptr(), scratch.data_ptr(), nbytes, _current_stream(dev))
+    if rc:
+        check(rc, "ttt_causal_conv_bwd")
+    return dx, dparams.as_strided((W, K), (K, 1)), dparams.as_strided((W,), (1,), W * K), dinit
 
 
-@_on_tensor_device
+@_on_device
 def causal_conv_step(x, state, weight, bias, activation, index):
     """One token per row: y [B, D]; state [slots, K - 1, D] shifted in place."""
-    _real(weight=weight, bias=bias)
+    _real("weight", weight), _real("bias", bias)
     _check_devices((x, state, weight, bias, index))
     act = _act_code(activation)
     if x.dim() != 2 or x.shape[1] < 1:

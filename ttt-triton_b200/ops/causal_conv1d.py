@@ -16,52 +16,51 @@ x: [B, L, D] in fp32, bf16 or fp16 (a view of a wider projection is read in plac
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 import _scan_core as core
 
 
 class CausalConv1d(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, init, act, seq, nseq, want_final):
-        ctx.set_materialize_grads(False)
-        ctx.param_dtypes = (weight.dtype, bias.dtype if bias is not None else None)
-        x, w, b = core._rows(x), core._f32(weight), core._f32(bias)
-        init = init.contiguous() if init is not None else None
-        y, fin = core.causal_conv_forward(x, w, b, act, init, seq, nseq, want_final)
-        ctx.act = act
+    def forward(ctx, x, w, b, init, seq, call):
+        act, sizes, nseq, want_final = call
+        y, fin, nbytes = core.causal_conv_forward(x, w, b, act, init, seq, nseq, want_final, sizes, True)
+        ctx.call = act, sizes, nbytes
         ctx.save_for_backward(x, w, b, init, seq)
+        if not want_final:
+            return y
+        ctx.set_materialize_grads(False)
         return y, fin
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dfin):
+    @core.first_order
+    def backward(ctx, dy, dfin=None):
         x, w, b, init, seq = ctx.saved_tensors
-        dy = torch.zeros(x.shape, device=x.device, dtype=x.dtype) if dy is None else dy.to(x.dtype).contiguous()
-        dfin = dfin.to(x.dtype).contiguous() if dfin is not None else None
-        dx, dw, db, dinit = core.causal_conv_backward(x, w, b, ctx.act, init, seq, dy, dfin, ctx.needs_input_grad[3])
-        dtypes = ctx.param_dtypes
-        return (dx, dw.to(dtypes[0]), db.to(dtypes[1]) if dtypes[1] is not None else None, dinit, None, None, None,
-                None)
+        act, sizes, nbytes = ctx.call
+        if dy is None or dy.dtype is not x.dtype or not dy.is_contiguous():
+            dy = core._upstream(dy, x)
+        if dfin is not None:
+            dfin = core._upstream(dfin, x)
+        dx, dw, db, dinit = core.causal_conv_backward(x, w, b, act, init, seq, dy, dfin,
+                                                      init is not None and ctx.needs_input_grad[3], sizes, nbytes)
+        return dx, dw, db if b is not None else None, dinit, None, None
 
 
 def causal_conv1d(x, weight, bias=None, activation=None, initial_state=None, cu_seqlens=None,
                   return_final_state=False):
     act = core._act_code(activation)
-    if x.dim() != 3:
-        raise ValueError(f"x must be [B, L, D], got shape {tuple(x.shape)}")
-    nseq, cu = core.packed(cu_seqlens, x)
-    core.check_conv(x, weight, bias, initial_state, nseq)
+    nseq, cu = core.packed(cu_seqlens, x) if cu_seqlens is not None else (x.shape[0], None)
+    sizes = core.check_conv(x, weight, bias, initial_state, nseq)
     seq = None
     if cu is not None:
         core.require_cuda(x, cu)
         seq = core.sequence_index(cu, x.shape[1])
-    if core.training(x, weight, bias, initial_state):
-        y, fin = CausalConv1d.apply(x, weight, bias, initial_state, act, seq, nseq, bool(return_final_state))
-    else:
-        init = initial_state.contiguous() if initial_state is not None else None
-        y, fin = core.causal_conv_forward(core._rows(x), core._f32(weight), core._f32(bias), act, init, seq, nseq,
-                                          bool(return_final_state))
+    # casts and copies, if any, are autograd's
+    x, w, b = core._rows(x), core._f32(weight), core._f32(bias)
+    init = initial_state.contiguous() if initial_state is not None else None
+    if core.training(x, w, b, init):
+        return CausalConv1d.apply(x, w, b, init, seq, (act, sizes, nseq, bool(return_final_state)))
+    y, fin, _ = core.causal_conv_forward(x, w, b, act, init, seq, nseq, bool(return_final_state), sizes, False)
     return (y, fin) if return_final_state else y
 
 

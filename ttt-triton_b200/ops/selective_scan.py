@@ -21,7 +21,6 @@ cu_seqlens, through the final state too; each gradient has its input's dtype.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 import _scan_core as core
 
@@ -35,7 +34,6 @@ def _layouts(u, delta, A, B, C, D, z, delta_bias):
 class SelectiveScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, u, delta, A, B, C, D, z, delta_bias, init, softplus, seq, nseq, want_final):
-        ctx.set_materialize_grads(False)
         ctx.param_dtypes = (A.dtype, D.dtype if D is not None else None,
                             delta_bias.dtype if delta_bias is not None else None,
                             init.dtype if init is not None else None)
@@ -43,22 +41,22 @@ class SelectiveScan(torch.autograd.Function):
         out, fin, saved = core.selective_scan_forward(*args, softplus, init, seq, nseq, want_final, True)
         ctx.softplus = softplus
         ctx.save_for_backward(*args, init, seq, saved)
+        if not want_final:
+            return out
+        ctx.set_materialize_grads(False)
         return out, fin
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dout, dfin):
+    @core.first_order
+    def backward(ctx, dout, dfin=None):
         *args, init, seq, saved = ctx.saved_tensors
-        u = args[0]
-        dout = torch.zeros(u.shape, device=u.device, dtype=u.dtype) if dout is None else dout.to(u.dtype).contiguous()
-        dfin = core._f32(dfin)
-        want_dinit = ctx.needs_input_grad[8]
+        dout, dfin = core._upstream(dout, args[0]), core._f32(dfin)
         du, ddelta, dA, dB, dC, dD, dz, dbias, dinit = core.selective_scan_backward(
-            *args, ctx.softplus, init, seq, saved, dout, dfin, want_dinit)
-        dtypes = ctx.param_dtypes
-        return (du, ddelta, dA.to(dtypes[0]), dB, dC, dD.to(dtypes[1]) if dtypes[1] is not None else None, dz,
-                dbias.to(dtypes[2]) if dtypes[2] is not None else None,
-                dinit.to(dtypes[3]) if dinit is not None else None, None, None, None, None)
+            *args, ctx.softplus, init, seq, saved, dout, dfin, ctx.needs_input_grad[8])
+        as_, dtypes = core._as, ctx.param_dtypes
+        return (du, ddelta, as_(dA, dtypes[0]), dB, dC, as_(dD, dtypes[1]) if dtypes[1] is not None else None, dz,
+                as_(dbias, dtypes[2]) if dtypes[2] is not None else None,
+                as_(dinit, dtypes[3]) if dinit is not None else None, None, None, None, None)
 
 
 def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_softplus=False, initial_state=None,
@@ -69,18 +67,17 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, delta_sof
         C = C.unsqueeze(2)
     if u.dim() != 3:
         raise ValueError(f"u must be [B, L, D], got shape {tuple(u.shape)}")
-    nseq, cu = core.packed(cu_seqlens, u)
+    nseq, cu = core.packed(cu_seqlens, u) if cu_seqlens is not None else (u.shape[0], None)
     core.check_scan(u, delta, A, B, C, D, z, delta_bias, initial_state, nseq)
     seq = None
     if cu is not None:
         core.require_cuda(u, cu)
         seq = core.sequence_index(cu, u.shape[1])
     if core.training(u, delta, A, B, C, D, z, delta_bias, initial_state):
-        out, fin = SelectiveScan.apply(u, delta, A, B, C, D, z, delta_bias, initial_state, bool(delta_softplus), seq,
-                                       nseq, bool(return_final_state))
-    else:
-        out, fin, _ = core.selective_scan_forward(*_layouts(u, delta, A, B, C, D, z, delta_bias), bool(delta_softplus),
-                                                  core._f32(initial_state), seq, nseq, bool(return_final_state), False)
+        return SelectiveScan.apply(u, delta, A, B, C, D, z, delta_bias, initial_state, bool(delta_softplus), seq, nseq,
+                                   bool(return_final_state))
+    out, fin, _ = core.selective_scan_forward(*_layouts(u, delta, A, B, C, D, z, delta_bias), bool(delta_softplus),
+                                              core._f32(initial_state), seq, nseq, bool(return_final_state), False)
     return (out, fin) if return_final_state else out
 
 
