@@ -8,6 +8,7 @@ import torch
 
 import ops
 import scan_reference as R
+from forecaster import SelectiveScanLayer
 from test_selective_scan_gpu import call, make
 
 pytestmark = pytest.mark.gpu
@@ -192,3 +193,18 @@ def test_an_output_or_a_final_state_alone():
         for s, p, q in zip(sums, *alone):
             p, q = (torch.zeros_like(s) if v is None else v for v in (p, q))
             assert R.rel(p + q, s) <= 2.0**-20
+
+
+# ------------------------------------------------------------------------------ the layer
+def test_the_layer_asks_for_states_only_where_they_are_wanted(monkeypatch):
+    asked = []
+    for name in ("causal_conv1d", "selective_scan"):
+        f = getattr(ops, name)
+        monkeypatch.setattr(ops, name, lambda *a, f=f: asked.append(a[-1]) or f(*a))
+    torch.manual_seed(0)
+    m = SelectiveScanLayer(16, act_dtype=torch.float32).to(DEV)
+    h = torch.randn(2, 9, 16, device=DEV)
+    out = m(h)
+    again, (rows, state) = m(h, return_state=True)
+    assert asked == [False, False, True, True]
+    assert torch.equal(out, again) and rows.shape == (2, 3, 32) and state.shape == (2, 32, 16)

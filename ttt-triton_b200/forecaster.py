@@ -195,10 +195,12 @@ class SelectiveScanLayer(nn.Module):
         dt = self.act_dtype
         x, z = Fn.linear(hidden_states.to(dt), self.in_proj.weight.to(dt)).chunk(2, -1)
         conv0, scan0 = state if state is not None else (None, None)
-        x, conv1 = ops.causal_conv1d(x, self.conv_weight, self.conv_bias, "silu", conv0, cu_seqlens, True)
+        x = ops.causal_conv1d(x, self.conv_weight, self.conv_bias, "silu", conv0, cu_seqlens, return_state)
+        x, conv1 = x if return_state else (x, None)
         delta, B, C = self._scan_inputs(x)
-        y, scan1 = ops.selective_scan(x, delta, -torch.exp(self.A_log), B, C, self.D, z, self.dt_proj.bias, True, scan0,
-                                      cu_seqlens, True)
+        y = ops.selective_scan(x, delta, -torch.exp(self.A_log), B, C, self.D, z, self.dt_proj.bias, True, scan0,
+                               cu_seqlens, return_state)
+        y, scan1 = y if return_state else (y, None)
         out = Fn.linear(y, self.out_proj.weight.to(dt))
         return (out, (conv1, scan1)) if return_state else out
 
