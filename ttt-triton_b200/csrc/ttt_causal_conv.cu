@@ -151,17 +151,18 @@ __device__ __forceinline__ void initial_rows(const Params& p, int s, int d, Vals
     hist[j] = p.init && s >= 0 ? unpack<T, VEC>(load<T, VEC>(p.init, ((long long)s * (K - 1) + K - 2 - j) * p.D + d))
                                : zeros<VEC>();
 }
-// The rows before token t0 > 0 of a run (of its sequence: `first` is its first token if that is
-// among them).
+// The rows before token t0 > 0 of a run, of its sequence. Returns the sequence's first token if that
+// is among them, else -K.
 template <typename T, int K, int VEC, bool SEQ>
-__device__ __forceinline__ void rows_before(const Params& p, const T* x, int t0, int d, int& first,
-                                            Vals<VEC> (&hist)[K - 1]) {
+__device__ __forceinline__ int rows_before(const Params& p, const T* x, int t0, int d, Vals<VEC> (&hist)[K - 1]) {
+  int first = -K;
 #pragma unroll
   for (int j = 0; j < K - 1; ++j) hist[j] = zeros<VEC>();
   for (int t = max(0, t0 - (K - 1)); t < t0; ++t) {
     if (SEQ && starts<SEQ>(p, t)) initial_rows<T, K, VEC>(p, p.seq[t], d, hist), first = t;
     push<K, VEC>(hist, unpack<T, VEC>(load<T, VEC>(x, t * p.x_l)));
   }
+  return first;
 }
 
 template <typename T, int K, int VEC, bool SEQ>
@@ -178,8 +179,7 @@ __global__ void __launch_bounds__(kWarps * 32) conv_fwd_kernel(const __grid_cons
   const T* x = static_cast<const T*>(p.x) + a.row * p.x_b + d;
   T* y = static_cast<T*>(p.y) + (long long)a.row * p.L * p.D + d;
   Vals<VEC> hist[K - 1];
-  int first = 0;
-  rows_before<T, K, VEC, SEQ>(p, x, a.t0, d, first, hist);
+  rows_before<T, K, VEC, SEQ>(p, x, a.t0, d, hist);
   const auto output = [&](const Vals<VEC>& v) {
     Vals<VEC> q = taps.at(v, hist);
     if (p.act)
@@ -234,8 +234,7 @@ __global__ void __launch_bounds__(kWarps * 32) conv_bwd_kernel(const __grid_cons
     const T* dy = static_cast<const T*>(p.dy) + (long long)a.row * p.L * p.D + d;
     T* dx = static_cast<T*>(p.dx) + (long long)a.row * p.L * p.D + d;
     Vals<VEC> hist[K - 1], acc[K];  // acc[j]: the gradient of the row j before
-    int first = -K;  // the sequence's first token, or any earlier place
-    rows_before<T, K, VEC, SEQ>(p, x, a.t0, d, first, hist);
+    int first = rows_before<T, K, VEC, SEQ>(p, x, a.t0, d, hist);  // the sequence's first token, or any earlier place
 #pragma unroll
     for (int j = 0; j < K; ++j) acc[j] = zeros<VEC>();
     const int stop = min(p.L, a.t1 + K - 1);

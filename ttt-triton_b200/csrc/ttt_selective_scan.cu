@@ -486,7 +486,7 @@ int chunk_states(const Params& p, int dt, bool rev, cudaStream_t st, const char*
                         : launch_chunks<float, false>(p, st, who);
 }
 
-// Whether stage_rows may read B and C four states at a time.
+// Whether Rows::fetch may read B and C four states at a time.
 bool quads(const Params& p, int dt) {
   const int elem = dt == DT_F32 ? 4 : 2;
   const Shape s = shape_of(p.N);
