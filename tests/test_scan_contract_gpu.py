@@ -118,8 +118,9 @@ def test_a_nonfinite_token_stays_out_of_its_neighbours_sums(dtype, N, G, value, 
 def test_bf16_sums_over_channels_round_as_fp32_ones():
     """dB and dC of bf16 inputs beside the 64-bit values rounded once. A value falls to the other
     side of a rounding border with the probability of its error over the step, 2^-8 of the value
-    at least. Summands rounded to 2^-17 give at most 2^-9 of all values, the recurrence's fp32
-    errors of some 2^-22 nothing beside that; 0.5 % are allowed (summands of 11 bits: 9 %)."""
+    at least. The recurrence's and the sums' fp32 errors of some 2^-22 of the terms, ten times that
+    of a sum in which random signs cancel, give 0.1 %; 0.5 % are allowed (summands rounded to 11
+    bits: 9 %)."""
     t = make(4, 100, 64, 16, 1, torch.bfloat16, 31)
     leaves = {k: v.to(DEV).requires_grad_(True) for k, v in t.items()}
     ref = {k: v.double().requires_grad_(True) for k, v in t.items()}

@@ -10,10 +10,12 @@
 // thread. Meanwhile the second part finishes the element-wise gradients of the tile before and
 // prepares the step sizes and gates of the next (one barrier a tile). Sums over a channel's
 // states (s1, s2 and y) pass through shared memory. Sums over channels (dB, dC): a thread adds
-// its two channels' products, and the tensor cores add over the threads, as products of the
-// matrix of those (16 states x 4 threads, one mma.sync a pair of states) with a vector of ones
-// in the column of the token and zeros in the others. The matrix takes bf16 numbers: a summand is
-// the sum of two (bf16 inputs, rounded to 2^-17) or three (fp16 and fp32, exact), added in fp32.
+// its two channels' products, the four threads that have the same states exchange theirs, and
+// the second part adds what warps and groups of lanes have. All in fp32, so that no token's
+// value meets another's: on the tensor cores, with one token a column, a non-finite value spoils
+// the columns beside it (zero times infinity), 16-bit operands need two or three parts, and the
+// conversions cost more than the exchanges: 16 x 2048 x 1536, 16 states, 1.19 ms against 1.27
+// (bf16 parts to 2^-17) and 1.55 (exact); 64 states 4 x 2048 x 1024 725 us against 827.
 // What the CTAs of a group have of dB and dC, and
 // what the rows and pieces have of dA, dD and dbias, is written as partials and added in a
 // fixed order afterwards, so that results do not depend on timing.
@@ -34,7 +36,6 @@ struct Bwd {
   static constexpr int RING = 4;                     // runs whose first states are on their way
   static constexpr int RUNS = LN >= 4 ? 2 : 1, TB = RUNS * SUB;  // tokens of a tile
   static constexpr int CG = 8 / LN;                  // groups of 8 channels in a warp
-  static constexpr int TS = LN < SUB ? LN : SUB;     // tokens side by side in a product's columns
   static constexpr int STEP = HELP / (DT / 2);       // tokens between a thread's couples of channels
   static constexpr int TWOS = (TB + STEP - 1) / STEP;
   static constexpr int YS = DT + (LN == 1 ? 0 : LN == 2 ? 16 : 8);  // row of partial sums, padded off bank conflicts
@@ -49,39 +50,23 @@ struct Bwd {
     Tile tile[2];
     float2 dA[MAIN * NPT], dD[HELP], dbias[HELP];    // sums over many tiles
     float4 kept[RING][MAIN * NPT / 2];               // states before the coming runs, each thread's own
-    float4 carry[MAIN * NPT / 2];                    // what enters the run from behind, each thread's own
   };
 };
 
-// Adds a pair of states' v over the 4 threads of a channel group to the column that `one` (two
-// bf16 ones, or zeros) marks. A value is the sum of bf16 numbers, its leading 8 bits, the next 8
-// and the rest, which the matrix takes as terms of their own: a thread has columns
-// 2 (lane % 4), + 1 (+ 8, + 9) of row lane / 4 for v.x and of 8 + lane / 4 for v.y.
-// EXACT: three parts, all 24 bits. Else two, the second rounded: 2^-17 of a value, which is 2^-8 of
-// the half step that dB and dC of bf16 inputs are rounded by (16 x 2048 x 1536, 16 states:
-// backward 1.27 ms, 1.55 ms with three parts). CHECK: an infinite v has no further parts (infinity less
-// infinity is not a number). The products are volatile: all 32 lanes have to execute them, and what
-// follows stores their results in some lanes only, where the compiler could otherwise move them.
-template <bool EXACT, bool CHECK>
-__device__ __forceinline__ void add_over_channels(float (&c)[4], float2 v, unsigned one) {
-  const auto lead = [](float2 x) {
-    return make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffff0000u), __uint_as_float(__float_as_uint(x.y) & 0xffff0000u));
+// Adds a token's products for dB and dC over the 4 threads of a channel group (the lanes that differ
+// in their last two bits), two exchanges that halve what a thread holds: it ends with the H / 2 pairs
+// of states from (l3 & 1) H / 2 on, of dB (l3 < 2) or dC.
+template <int H>
+__device__ __forceinline__ void add_over_channels(const float2 (&vB)[H], const float2 (&vC)[H], int l3, float2 (&sum)[H / 2]) {
+  const auto other = [](float2 x, int lanes) {
+    return make_float2(__shfl_xor_sync(0xffffffffu, x.x, lanes), __shfl_xor_sync(0xffffffffu, x.y, lanes));
   };
-  const auto both = [](float x, unsigned r) { return __byte_perm(__float_as_uint(x), r, 0x7632); };  // the two leads
-  const float2 h = lead(v);
-  float2 r = __ffma2_rn(h, all2(-1.f), v);
-  if constexpr (CHECK) r = make_float2(fabsf(h.x) < INFINITY ? r.x : 0.f, fabsf(h.y) < INFINITY ? r.y : 0.f);
-  if constexpr (EXACT) {
-    const float2 l = __ffma2_rn(lead(r), all2(-1.f), r);
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%8}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(both(v.x, __float_as_uint(r.x))), "r"(both(v.y, __float_as_uint(r.y))), "r"(__float_as_uint(l.x)),
-          "r"(__float_as_uint(l.y)), "r"(one));
-  } else {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(both(v.x, __float_as_uint(r.x) + 0x8000u)), "r"(both(v.y, __float_as_uint(r.y) + 0x8000u)), "r"(one));
-  }
+  float2 half[H];
+#pragma unroll
+  for (int j = 0; j < H; ++j) half[j] = __fadd2_rn(l3 & 2 ? vC[j] : vB[j], other(l3 & 2 ? vB[j] : vC[j], 2));
+#pragma unroll
+  for (int j = 0; j < H / 2; ++j)
+    sum[j] = __fadd2_rn(l3 & 1 ? half[j + H / 2] : half[j], other(l3 & 1 ? half[j] : half[j + H / 2], 1));
 }
 
 // Barrier ID of the CTA's first THREADS (or of its second part), waited for at places of its own.
@@ -93,7 +78,6 @@ __device__ __forceinline__ void part_barrier() {
 template <typename T, int LN, int NPT, bool SEQ, bool TWO>
 __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const __grid_constant__ Params p) {
   using F = Bwd<LN, NPT>;
-  constexpr bool EXACT = !std::is_same<T, __nv_bfloat16>::value;
   constexpr int H = NPT / 2;
   extern __shared__ __align__(16) unsigned char raw_smem[];
   auto& s = *reinterpret_cast<typename F::Smem*>(raw_smem);
@@ -105,11 +89,13 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
 
   if (threadIdx.x < F::MAIN) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // lane -> states and channels, as the sums over channels want them: rows lane / 4 of the
-    // matrix are (channel group, state run), columns lane % 4 the two channels' threads
+    // lane -> states and channels, as the sums over channels want them: lane / 4 is (channel
+    // group, run of states), lane % 4 one of the threads whose sums are added
     const int l3 = lane & 3, row8 = lane >> 2, cg = row8 / LN, nl = row8 % LN, n0 = nl * NPT;
     const int cl = warp * F::CW + 8 * cg + 2 * l3;
-    const int col_tok = row8 / F::CG;  // and the token of this thread's column of the sums
+    // what this thread has of a token's sums over channels: of dB or dC, from dB's first on
+    const int sums = (l3 & 2 ? F::WARPS * F::CG * F::TB * F::NP : 0) + (warp * F::CG + cg) * F::TB * F::NP + n0 +
+                     (l3 & 1) * H;
     const int d = w.g * p.Dg + w.d0 + cl;
     const bool c0 = w.d0 + cl < p.Dg, c1 = w.d0 + cl + 1 < p.Dg;
     const float* kept = p.hsave + (long long)w.row * p.nsave * DN;
@@ -168,14 +154,10 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
       for (int t0 = tt + (F::RUNS - 1) * F::SUB; t0 >= tt; t0 -= F::SUB) {
         if (t0 >= tend) continue;
         const int b = t0 - tt;
-        // The run's tokens. Without CHECK, whether its sums over channels are all finite: a product of
-        // several tokens has zeros in the columns of the others, and zero times a non-finite value
-        // spoils them. The run is then taken `again`, with a product for each token.
-        const auto tokens = [&](auto checks, bool again) {
+        const auto tokens = [&](auto checks) {
           constexpr bool CHECK = decltype(checks)::value;
           float2 a[F::SUB][2][H], ah[F::SUB][2][H];
-          float total = 0.f;
-          if (!again) asm volatile("cp.async.wait_group %0;" ::"n"(F::RING - 2) : "memory");
+          asm volatile("cp.async.wait_group %0;" ::"n"(F::RING - 2) : "memory");
           Both<NPT> h;
 #pragma unroll
           for (int c = 0; c < 2; ++c)
@@ -184,15 +166,8 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
               const float4 q = s.kept[run % F::RING][tid + (c * (NPT / 4) + e) * F::MAIN];
               h.c[c].v[2 * e] = make_float2(q.x, q.y), h.c[c].v[2 * e + 1] = make_float2(q.z, q.w);
             }
-          if (!CHECK) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int e = 0; e < NPT / 4; ++e)
-                s.carry[tid + (c * (NPT / 4) + e) * F::MAIN] =
-                    make_float4(carry.c[c].v[2 * e].x, carry.c[c].v[2 * e].y, carry.c[c].v[2 * e + 1].x, carry.c[c].v[2 * e + 1].y);
-          }
-          if (!again) fetch_states(run - (F::RING - 1));
+          fetch_states(run - (F::RING - 1));
+          --run;
 #pragma unroll
           for (int k = 0; k < F::SUB; ++k) {
             if constexpr (CHECK && SEQ) {
@@ -212,92 +187,57 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
                 h.c[c].v[j] = __ffma2_rn(all2(c ? d4.w : d4.y), B2.v[j], ah[k][c][j]);
               }
           }
-          constexpr int TS = CHECK ? 1 : F::TS;
 #pragma unroll
-          for (int g0 = F::SUB - TS; g0 >= 0; g0 -= TS) {
-            float accB[H][4], accC[H][4];
-#pragma unroll
-            for (int j = 0; j < H; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) accB[j][e] = accC[j][e] = 0.f;
-#pragma unroll
-            for (int k = g0 + TS - 1; k >= g0; --k) {
-              if constexpr (CHECK) {
-                if (t0 + k >= tend) continue;
-                if (SEQ && (mask.end >> (b + k) & 1)) {
-                  const int sq = p.seq[t0 + k];
-                  carry = load2(p.dfin + sq * DN, sq >= 0 && p.dfin);
-                }
-              }
-              const float4 d4 = *reinterpret_cast<const float4*>(&tile.d[(b + k) * F::DT + cl]);
-              const float2 dy2 = *reinterpret_cast<const float2*>(&tile.dy[(b + k) * F::DT + cl]);
-              const Pairs<NPT> B2 = row_pairs<NPT>(tile.B + (b + k) * F::NP + n0), C2 = row_pairs<NPT>(tile.C + (b + k) * F::NP + n0);
-              const unsigned one = col_tok == k - g0 ? 0x3f803f80u : 0u;
-              const float2 zero = all2(0.f);
-              float2 s1[2] = {zero, zero}, s2[2] = {zero, zero}, s3[2] = {zero, zero};
-#pragma unroll
-              for (int j = 0; j < H; ++j) {
-                float2 g[2], hn[2];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                  const float2 ahj = ah[k][c][j];
-                  g[c] = __ffma2_rn(C2.v[j], all2(c ? dy2.y : dy2.x), carry.c[c].v[j]);
-                  hn[c] = __ffma2_rn(all2(c ? d4.w : d4.y), B2.v[j], ahj);
-                  const float2 q = __fmul2_rn(g[c], ahj);
-                  s1[c] = j ? __ffma2_rn(g[c], B2.v[j], s1[c]) : __fmul2_rn(g[c], B2.v[j]);
-                  s2[c] = j ? __ffma2_rn(q, A2.c[c].v[j], s2[c]) : __fmul2_rn(q, A2.c[c].v[j]);
-                  s3[c] = j ? __ffma2_rn(hn[c], C2.v[j], s3[c]) : __fmul2_rn(hn[c], C2.v[j]);
-                  if (!CHECK || !again) dA.c[c].v[j] = __ffma2_rn(q, all2(c ? d4.z : d4.x), dA.c[c].v[j]);
-                  carry.c[c].v[j] = __fmul2_rn(a[k][c][j], g[c]);
-                }
-                add_over_channels<EXACT, CHECK>(accB[j], __ffma2_rn(g[0], all2(d4.y), __fmul2_rn(g[1], all2(d4.w))), one);
-                add_over_channels<EXACT, CHECK>(accC[j], __ffma2_rn(hn[0], all2(dy2.x), __fmul2_rn(hn[1], all2(dy2.y))), one);
-              }
-              const int o = ((b + k) * LN + nl) * F::YS + cl;
-              *reinterpret_cast<float2*>(&tile.s1[o]) = make_float2(s1[0].x + s1[0].y, s1[1].x + s1[1].y);
-              *reinterpret_cast<float2*>(&tile.s2[o]) = make_float2(s2[0].x + s2[0].y, s2[1].x + s2[1].y);
-              *reinterpret_cast<float2*>(&tile.s3[o]) = make_float2(s3[0].x + s3[0].y, s3[1].x + s3[1].y);
-              if constexpr (CHECK && SEQ) {
-                if (p.dinit && (mask.start >> (b + k) & 1)) {
-                  const int sq = p.seq[t0 + k];
-                  store_both<NPT>(p.dinit + sq * DN, d, n0, p.N, sq >= 0 && c0, sq >= 0 && c1, carry);
-                }
+          for (int k = F::SUB - 1; k >= 0; --k) {
+            if constexpr (CHECK) {
+              if (t0 + k >= tend) continue;
+              if (SEQ && (mask.end >> (b + k) & 1)) {
+                const int sq = p.seq[t0 + k];
+                carry = load2(p.dfin + sq * DN, sq >= 0 && p.dfin);
               }
             }
-            if (!CHECK) {  // one of this lane's two columns: what is not finite is in all
+            const float4 d4 = *reinterpret_cast<const float4*>(&tile.d[(b + k) * F::DT + cl]);
+            const float2 dy2 = *reinterpret_cast<const float2*>(&tile.dy[(b + k) * F::DT + cl]);
+            const Pairs<NPT> B2 = row_pairs<NPT>(tile.B + (b + k) * F::NP + n0), C2 = row_pairs<NPT>(tile.C + (b + k) * F::NP + n0);
+            const float2 zero = all2(0.f);
+            float2 vB[H], vC[H], s1[2] = {zero, zero}, s2[2] = {zero, zero}, s3[2] = {zero, zero};
 #pragma unroll
-              for (int j = 0; j < H; ++j) total += accB[j][0] + accB[j][2] + (accC[j][0] + accC[j][2]);
+            for (int j = 0; j < H; ++j) {
+              float2 g[2], hn[2];
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const float2 ahj = ah[k][c][j];
+                g[c] = __ffma2_rn(C2.v[j], all2(c ? dy2.y : dy2.x), carry.c[c].v[j]);
+                hn[c] = __ffma2_rn(all2(c ? d4.w : d4.y), B2.v[j], ahj);
+                const float2 q = __fmul2_rn(g[c], ahj);
+                s1[c] = j ? __ffma2_rn(g[c], B2.v[j], s1[c]) : __fmul2_rn(g[c], B2.v[j]);
+                s2[c] = j ? __ffma2_rn(q, A2.c[c].v[j], s2[c]) : __fmul2_rn(q, A2.c[c].v[j]);
+                s3[c] = j ? __ffma2_rn(hn[c], C2.v[j], s3[c]) : __fmul2_rn(hn[c], C2.v[j]);
+                dA.c[c].v[j] = __ffma2_rn(q, all2(c ? d4.z : d4.x), dA.c[c].v[j]);
+                carry.c[c].v[j] = __fmul2_rn(a[k][c][j], g[c]);
+              }
+              vB[j] = __ffma2_rn(g[0], all2(d4.y), __fmul2_rn(g[1], all2(d4.w)));
+              vC[j] = __ffma2_rn(hn[0], all2(dy2.x), __fmul2_rn(hn[1], all2(dy2.y)));
             }
-            // of the products' two columns in this lane, those of the row's own channel group
+            float2 sum[H / 2];
+            add_over_channels<H>(vB, vC, l3, sum);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int c = 2 * l3 + e, tc = c / F::CG;
-              if (c % F::CG == cg && tc < TS) {
-                const int o = (b + g0 + tc) * F::NP + n0;
-#pragma unroll
-                for (int j = 0; j < H; ++j) {
-                  *reinterpret_cast<float2*>(&tile.dB[warp * F::CG + cg][o + 2 * j]) = make_float2(accB[j][e], accB[j][2 + e]);
-                  *reinterpret_cast<float2*>(&tile.dC[warp * F::CG + cg][o + 2 * j]) = make_float2(accC[j][e], accC[j][2 + e]);
-                }
+            for (int j = 0; j < H / 2; ++j)
+              *reinterpret_cast<float2*>(&tile.dB[0][sums + (b + k) * F::NP + 2 * j]) = sum[j];
+            const int o = ((b + k) * LN + nl) * F::YS + cl;
+            *reinterpret_cast<float2*>(&tile.s1[o]) = make_float2(s1[0].x + s1[0].y, s1[1].x + s1[1].y);
+            *reinterpret_cast<float2*>(&tile.s2[o]) = make_float2(s2[0].x + s2[0].y, s2[1].x + s2[1].y);
+            *reinterpret_cast<float2*>(&tile.s3[o]) = make_float2(s3[0].x + s3[0].y, s3[1].x + s3[1].y);
+            if constexpr (CHECK && SEQ) {
+              if (p.dinit && (mask.start >> (b + k) & 1)) {
+                const int sq = p.seq[t0 + k];
+                store_both<NPT>(p.dinit + sq * DN, d, n0, p.N, sq >= 0 && c0, sq >= 0 && c1, carry);
               }
             }
           }
-          return fabsf(total) < INFINITY;
         };
-        bool careful = t0 + F::SUB > tend || (SEQ && ((mask.start | mask.end) >> b & ((1u << F::SUB) - 1)));
-        bool again = false;
-        if (!careful && !__all_sync(0xffffffffu, tokens(std::false_type{}, false))) {
-          careful = again = true;
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int e = 0; e < NPT / 4; ++e) {
-              const float4 q = s.carry[tid + (c * (NPT / 4) + e) * F::MAIN];
-              carry.c[c].v[2 * e] = make_float2(q.x, q.y), carry.c[c].v[2 * e + 1] = make_float2(q.z, q.w);
-            }
-        }
-        if (careful) tokens(std::true_type{}, again);
-        --run;
+        if (t0 + F::SUB > tend || (SEQ && ((mask.start | mask.end) >> b & ((1u << F::SUB) - 1)))) tokens(std::true_type{});
+        else tokens(std::false_type{});
       }
       if (i % 8 == 7 || i + 1 == ntiles) {  // short sums first: a long chain of additions loses bits
 #pragma unroll
