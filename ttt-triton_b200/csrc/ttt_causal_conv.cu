@@ -4,9 +4,12 @@
 //
 // Rows before a sequence's first token are its initial state's K - 1 rows, or zero; the final
 // state is its last K - 1 rows. It moves every value once in and once out with a handful of
-// operations each, so memory bounds it: a thread holds VEC adjacent channels (a vector load
+// operations each, so memory is its floor: a thread holds VEC adjacent channels (a vector load
 // per token), walks a run of tokens with the last K - 1 rows in registers, and loads several
-// tokens ahead; a warp covers 32 adjacent vectors of one run, a block 8 runs.
+// tokens together; a warp covers 32 adjacent vectors of one run, a block 8 runs. Measured, 32 x
+// 4096 x 1024 bf16, K = 4, silu: 150 us forward (3.6 TB/s), 240 us backward (3.4 TB/s). The latency of
+// those loads bounds it: 14 warps an SM issue 1.1 to 1.3 instructions a clock and wait for global
+// memory most of the rest, as nothing is on its way while a block of tokens is worked on.
 //
 // Backward, dp = dy act'(p): dx[t] = sum_k w[k] dp[t + K - 1 - k], dw[k] = sum dp x, db = sum
 // dp. One walk forward in time: each dp is added to the gradients of the K rows that it

@@ -6,9 +6,10 @@
 // inputs are worked out once per (token, channel) into shared memory, then every thread runs
 // its states through the tile's tokens, then the partial outputs of a channel's threads are
 // added, the skip and the gate applied and the result written. One exponential per (token,
-// channel, state) is what bounds it, and next to that the shared-memory reads, whose cost is
-// bytes per thread whether or not threads read the same: the second channel halves those of
-// B and C.
+// channel, state) is its floor; the unit is half busy, and the fixed latency of the recurrence's
+// instructions at 24 warps an SM bounds it (16 x 2048 x 1536, 16 states: 408 us, floor 179).
+// Shared-memory reads cost bytes per thread whether or not threads read the same: the second
+// channel halves those of B and C.
 //
 // With few channels in all, the time axis is split into pieces: a first pass finds each
 // piece's end state from zero and the sum of its step sizes (its whole decay is
@@ -513,8 +514,8 @@ bool couples(const Params& p, int dt) {
 // main pass's time, about 128 tokens' worth of launches and 3 a piece; it pays where the `blocks` CTAs of
 // whole rows leave SMs empty, or a last round of them nearly so. An SM runs `resident` CTAs at
 // once; k of them take 0.4 + 0.6 k / resident of that time. Measured, 16 x 2048 x 1536 states
-// of 16: backward 1.32 ms whole (384 CTAs on 296 places), 1.44 ms in 3 pieces, whose first pass
-// alone takes 0.29 ms; 32 x 336 x 512 training 420 us in 4 pieces, 225 us whole; 1 x 8192 x 1024
+// of 16: backward 1.19 ms whole (384 CTAs on 296 places), 1.30 ms in 3 pieces, whose first pass
+// alone takes 0.29 ms; 32 x 336 x 512 training 305 us in 3 or 4 pieces, 209 us whole; 1 x 8192 x 1024
 // prompt 160 us in 128 pieces, 123 us in 26.
 int piece_tokens(long long blocks, int L, int resident, float extra) {
   const long long sms = sm_count(), places = sms * resident;
