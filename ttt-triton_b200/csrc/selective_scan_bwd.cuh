@@ -44,7 +44,7 @@ struct Bwd {
     float2 d[TB * DT];                               // step size, step size * input
     float dy[TB * DT];
     float s1[TB * LN * YS], s2[TB * LN * YS], s3[TB * LN * YS];
-    float dB[WARPS * CG][TB * NP], dC[WARPS * CG][TB * NP];
+    float sums[2 * WARPS * CG * TB * NP];            // over a group's channels: dB of all groups, dC of all
   };
   struct Smem {
     Tile tile[2];
@@ -93,9 +93,8 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
     // group, run of states), lane % 4 one of the threads whose sums are added
     const int l3 = lane & 3, row8 = lane >> 2, cg = row8 / LN, nl = row8 % LN, n0 = nl * NPT;
     const int cl = warp * F::CW + 8 * cg + 2 * l3;
-    // what this thread has of a token's sums over channels: of dB or dC, from dB's first on
-    const int sums = (l3 & 2 ? F::WARPS * F::CG * F::TB * F::NP : 0) + (warp * F::CG + cg) * F::TB * F::NP + n0 +
-                     (l3 & 1) * H;
+    // where this thread's part of a token's sums over channels lies
+    const int sums = ((l3 >> 1) * F::WARPS * F::CG + warp * F::CG + cg) * F::TB * F::NP + n0 + (l3 & 1) * H;
     const int d = w.g * p.Dg + w.d0 + cl;
     const bool c0 = w.d0 + cl < p.Dg, c1 = w.d0 + cl + 1 < p.Dg;
     const float* kept = p.hsave + (long long)w.row * p.nsave * DN;
@@ -223,7 +222,7 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
             add_over_channels<H>(vB, vC, l3, sum);
 #pragma unroll
             for (int j = 0; j < H / 2; ++j)
-              *reinterpret_cast<float2*>(&tile.dB[0][sums + (b + k) * F::NP + 2 * j]) = sum[j];
+              *reinterpret_cast<float2*>(&tile.sums[sums + (b + k) * F::NP + 2 * j]) = sum[j];
             const int o = ((b + k) * LN + nl) * F::YS + cl;
             *reinterpret_cast<float2*>(&tile.s1[o]) = make_float2(s1[0].x + s1[0].y, s1[1].x + s1[1].y);
             *reinterpret_cast<float2*>(&tile.s2[o]) = make_float2(s2[0].x + s2[0].y, s2[1].x + s2[1].y);
@@ -347,7 +346,8 @@ __global__ void __launch_bounds__(256, NPT == 4 ? 2 : 1) scan_bwd_kernel(const _
         if (tl + t < tend && n < p.N) {
           float vb = 0.f, vc = 0.f;
 #pragma unroll
-          for (int e = 0; e < F::WARPS * F::CG; ++e) vb += tile.dB[e][k], vc += tile.dC[e][k];
+          for (int e = 0; e < F::WARPS * F::CG; ++e)
+            vb += tile.sums[e * F::TB * F::NP + k], vc += tile.sums[(F::WARPS * F::CG + e) * F::TB * F::NP + k];
           if (SEQ && seq[tl + t] < 0) vb = vc = 0.f;
           part_B[t * part_step + n] = vb, part_C[t * part_step + n] = vc;
         }
