@@ -42,3 +42,11 @@ def test_state_layouts():
                          (torch.zeros(3, 1, 16)[..., ::2], (1, 8))):
         with pytest.raises(ValueError):
             check(state, shape)
+
+
+def test_shapes_that_are_no_batches():
+    for x in (torch.zeros(()), torch.zeros(8), torch.zeros(2, 3, 4, 8)):
+        with pytest.raises(ValueError, match=r"\[B, L, D\]"):
+            ops.causal_conv1d(x, torch.zeros(8, 3))
+        with pytest.raises(ValueError, match=r"\[B, L, D\]"):
+            ops.selective_scan(x, x, torch.zeros(8, 4), torch.zeros(1, 4, 4), torch.zeros(1, 4, 4))

@@ -77,7 +77,7 @@ _Strides2 = ctypes.c_longlong * 2
 def _f32(t):
     if t is None:
         return None
-    return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
+    return t if t.dtype is torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
 
 
 def _as(t, dtype):
@@ -317,7 +317,7 @@ def _check_taps(weight, bias, W):
 
 
 def _conv_sizes(x, weight, bias, init, nseq):
-    """(rows, L, D, K, type code) of a call, or what is wrong with it."""
+    """(rows, L, D, K, type code) of a call, or what is wrong with it. nseq: packed sequences, or None."""
     if x.dim() != 3:
         raise ValueError(f"x must be [B, L, D], got shape {tuple(x.shape)}")
     _real("weight", weight), _real("bias", bias)
@@ -326,7 +326,7 @@ def _conv_sizes(x, weight, bias, init, nseq):
     if shape[2] < 1:
         raise ValueError(f"x must be [B, L, D], got shape {tuple(shape)}")
     K = _check_taps(weight, bias, shape[2])
-    _shaped("initial_state", init, (nseq, K - 1, shape[2]))
+    _shaped("initial_state", init, (shape[0] if nseq is None else nseq, K - 1, shape[2]))
     _same(x, initial_state=init)
     return (*shape, K, dt)
 

@@ -49,12 +49,15 @@ class CausalConv1d(torch.autograd.Function):
 def causal_conv1d(x, weight, bias=None, activation=None, initial_state=None, cu_seqlens=None,
                   return_final_state=False):
     act = core._act_code(activation)
-    nseq, cu = core.packed(cu_seqlens, x) if cu_seqlens is not None else (x.shape[0], None)
+    seq = nseq = None
+    if cu_seqlens is not None:
+        nseq, cu = core.packed(cu_seqlens, x)
     sizes = core.check_conv(x, weight, bias, initial_state, nseq)
-    seq = None
-    if cu is not None:
+    if cu_seqlens is not None:
         core.require_cuda(x, cu)
-        seq = core.sequence_index(cu, x.shape[1])
+        seq = core.sequence_index(cu, sizes[1])
+    else:
+        nseq = sizes[0]
     # casts and copies, if any, are autograd's
     x, w, b = core._rows(x), core._f32(weight), core._f32(bias)
     init = initial_state.contiguous() if initial_state is not None else None
